@@ -277,7 +277,7 @@ def _plain_plan(s):
     owned.copy_(torch.where(takes, page, torch.where(fresh, -1, owned)))
     forks = forks & row_served
     got = page.gather(1, part.clamp(max=P - 1)[:, None])[:, 0]
-    copies = torch.where(forks[:, None], torch.stack([old, got], 1), -1)
+    copies = torch.where(forks[:, None], torch.stack([old, got, row_kv % ps], 1), -1)
     # rows: the tokens of a group (of each of its beams), one after another
     granted = torch.where(served, n, 0)
     starts = start if shared else (start[:, None] + n[:, None] * torch.arange(W, device=DEV)).flatten()
