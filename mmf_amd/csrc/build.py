@@ -22,6 +22,9 @@ LIB = os.path.join(os.path.dirname(HERE), "libmmf_amd.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
+    # no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on gfx950 now and then
+    # (the host pass does not know the feature and warns; harmless)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wno-unused-result", "-I", INCLUDE, "-I", HERE,
 ] + os.environ.get("MMF_AMD_EXTRA_HIPCC_FLAGS", "").split()     # e.g. -DMMF_WIDE_ABLATE for tools/wide_ablate.py
 
