@@ -746,6 +746,90 @@ int mmf_probe_mfma16(const void* a, const void* b, float* d, void* stream);   /*
 int mmf_probe_mfma32(const void* a, const void* b, float* d, void* stream);   /* out 64x16 */
 int mmf_probe_tr16(const void* lds_image_2048_bf16, const int* byte_addr_per_lane, void* out_64x4_bf16, void* stream);
 
+/* ---- decoding with a paged key / value cache and beams --------------------------------------------
+ * M4C decodes greedily and re-runs its whole multimodal transformer per step (mmf/models/m4c.py:284-304); the reference's BeamSearch
+ * (mmf/utils/text.py) selects on the host.  These entries keep the whole step on the device: the plan of a step (pages, slots), the write of
+ * the new keys and values, attention of the new tokens over the pages, the selection, the block tables after it.
+ *
+ * A cache is a pool of pages of `page_size` tokens (a power of two, 1 .. 1024) per layer, keys and values alike: element (page, head, pos, e) at
+ * page * page_stride + head * head_stride + pos * pos_stride + e.  A block table [rows, blocks] holds the pages of a row's sequence: token t of
+ * row r is in page tables[r][t / page_size] at position t % page_size.  Rows come in groups of `beams` (1 .. 32) that have the same length.
+ * Lengths, tables and lists are int32 on the device; the host never has to know them.  An index outside its table is left out and reported by
+ * mmf_amd_take_index_error(). */
+#define MMF_BEAMS_MAX 32
+#define MMF_PAGE_MAX 1024
+/* The plan of a step.  q_lens[g]: new tokens of each row of group g (shared: of the group, whose rows all see them); < 0: the group is done, the
+ * pages its rows own go back on the free stack and its length becomes 0.  kv_lens[g]: tokens in the cache.  Pages are taken from the top of the
+ * stack free_pages[0 .. free_top) in the order of rows and blocks.  shared: the group's first row gets the pages, the other rows' tables point to
+ * them (a prompt).  Not shared: every row gets pages of its own, and a row that is still sharing the block it goes on writing gets a page for it and a
+ * line in copies (source page, new page, tokens; else -1): run mmf_paged_copy before the write.  A group is served whole or not at all (`refused` counts those that wait):
+ * it waits if its tokens do not fit its table row or `rows`, or if it and the groups before it need more pages than there are.
+ * Outputs: q_start [rows of the plan = groups (shared) or groups * beams] first token row of each; granted [groups] new tokens that were
+ * planned; kv_out [groups] new lengths (may be kv_lens); slots [rows] page * page_size + position, positions [rows] position in the
+ * sequence, both -1 for the tokens of a group that waits and for rows behind the last; top_out (may be free_top). */
+typedef struct mmf_paged_plan_desc {
+    const int32_t* q_lens; const int32_t* kv_lens;
+    int32_t* tables; int32_t* owned;             /* [groups * beams, blocks]; owned: the page each row took for each of its blocks, -1 none */
+    int32_t* free_pages; const int32_t* free_top;
+    int32_t* q_start; int32_t* granted; int32_t* kv_out; int64_t* slots; int32_t* positions; int32_t* copies /* [groups * beams, 3] */; int32_t* top_out; int32_t* refused;
+    void* ws;                                    /* mmf_paged_plan_ws_bytes(groups) bytes, 16-byte aligned */
+    int groups, beams, blocks, page_size, rows, shared, free_capacity;
+} mmf_paged_plan_desc;
+int64_t mmf_paged_plan_ws_bytes(int groups);
+int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream);
+/* k / v row t, head h at t * k_row + h * k_head (elements) -> slot slots[t] of the caches; slots[t] < 0: skipped.  bf16 or fp32 throughout. */
+typedef struct mmf_paged_write_desc {
+    const void* k; const void* v; int64_t k_row, k_head, v_row, v_head;
+    void* k_cache; void* v_cache; int64_t page_stride, head_stride, pos_stride;
+    const int64_t* slots;
+    int tokens, pages, page_size, kv_heads, head_dim, is_f32;
+} mmf_paged_write_desc;
+int mmf_paged_write(const mmf_paged_write_desc* d, void* stream);
+/* Attention of new tokens over the pages of their row, whose last q_lens tokens are the new ones (already written):
+ *   out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j],  j < kv (causal: j <= kv - q_len + i),  query head h reads key head h / (heads / kv_heads).
+ * Row r: queries q_start[r] .. + q_lens[r / beams], keys kv_lens[r / beams].  A token that sees no key gives zeros; rows of `out` no request names are left
+ * as they were.  head_dim 64 or 128; bf16 (probabilities rounded to bf16 for the second product) or fp32 throughout; softmax statistics and sums fp32.
+ * max_q: no request has more new tokens.  ws: mmf_paged_attention_ws_bytes(d) bytes, 16-byte aligned (0: none needed). */
+typedef struct mmf_paged_attn_desc {
+    const void* q; int64_t q_row, q_head;
+    const void* k_cache; const void* v_cache; int64_t page_stride, head_stride, pos_stride;
+    const int32_t* tables; int64_t table_row;    /* elements between the table rows of consecutive requests */
+    const int32_t* kv_lens; const int32_t* q_start; const int32_t* q_lens;
+    void* out; int64_t out_row, out_head;
+    void* ws;
+    int tokens, requests, beams, blocks, pages, page_size, heads, kv_heads, head_dim, max_q, causal, is_f32;
+    float scale;
+} mmf_paged_attn_desc;
+int64_t mmf_paged_attention_ws_bytes(const mmf_paged_attn_desc* d);
+int mmf_paged_attention(const mmf_paged_attn_desc* d, void* stream);
+/* The best `beams` continuations of each group over beams x vocabulary (the reference's BeamSearch, mmf/utils/text.py): candidate (w, v) at scores[w] + log_softmax(logits[w])[v], of a finished beam only the
+ * end token at scores[w].  Descending; the lowest w * vocab + v first among equals.  NaN logits and scores count as -inf; so does every logit of a row that
+ * holds +inf.  finished_out = finished[parent] or token == eos.  history (optional) [groups, beams, length]: rows of the parents, column `step` the new
+ * tokens.  Every output may be its input.  logits bf16 or fp32, row stride ld. */
+typedef struct mmf_beam_select_desc {
+    const void* logits; int64_t ld;
+    const float* scores; const uint8_t* finished; const int64_t* history;
+    float* scores_out; int64_t* parents; int64_t* tokens; uint8_t* finished_out; int64_t* history_out;
+    void* ws;                                    /* mmf_beam_select_ws_bytes(groups, beams, vocab) bytes, 16-byte aligned */
+    int64_t vocab, eos, length, step;
+    int groups, beams, is_f32;
+} mmf_beam_select_desc;
+int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab);
+int mmf_beam_select(const mmf_beam_select_desc* d, void* stream);
+/* Tables after a selection: row w of a group becomes row parents[w]; the first child of a row keeps its unfinished block's page, every other child gets the page
+ * of a row without children and a line in copies [groups * beams, 3] (source, destination, tokens; else -1) for mmf_paged_copy.  tables_out may be tables. */
+typedef struct mmf_paged_reorder_desc {
+    const int64_t* parents; const int32_t* kv_lens; const int32_t* tables; int32_t* tables_out; int32_t* copies;
+    int groups, beams, blocks, page_size;
+} mmf_paged_reorder_desc;
+int mmf_paged_reorder(const mmf_paged_reorder_desc* d, void* stream);
+/* copies[r] = (source page, destination page, tokens): that many tokens of the page, in each of `planes` pools plane_stride elements apart. */
+typedef struct mmf_paged_copy_desc {
+    const int32_t* copies; void* cache; int64_t plane_stride, page_stride, head_stride, pos_stride;
+    int rows, planes, pages, page_size, kv_heads, head_dim, is_f32;
+} mmf_paged_copy_desc;
+int mmf_paged_copy(const mmf_paged_copy_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1529,11 +1529,14 @@ int mmf_layernorm_bwd_din(const void* dy, const void* x, const float* mean, cons
                               DropoutCfg{in_key, in_thr16, in_scale, in_seed}, stream);
 }
 
+int mmf_decode_take_error(void);
+int mmf_paged_attention_take_error(void);
 int mmf_amd_take_index_error(void) {
     int v = 0;
     if (hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_index_error), sizeof(int)) != hipSuccess) { mmf_amd_set_error("take_index_error: copy failed"); return -1; }
     if (v) { const int z = 0; (void)hipMemcpyToSymbol(HIP_SYMBOL(g_index_error), &z, sizeof(int)); }
-    return v;
+    const int dec = mmf_decode_take_error(), att = mmf_paged_attention_take_error();      // the paged cache's flags (paged_common.h)
+    return dec < 0 || att < 0 ? -1 : (v | dec | att);
 }
 
 int mmf_embed_text_fwd(const int64_t* ids, const int64_t* seg, const float* word, const float* pos, const float* type, void* y,
