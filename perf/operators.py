@@ -316,12 +316,15 @@ def _own_write(s):
 
 
 def _plain_write(s):
-    kc, vc, ps = s["key_cache"], s["value_cache"], s["case"]["page"]
-    keep = s["slots"] >= 0
+    kc, vc, slots = s["key_cache"], s["value_cache"], s["slots"]
+    pages, H, ps, D = kc.shape
+    # the token of each slot, if any: rows that are left out meet in a cell behind the last
+    token = torch.full((pages * ps + 1,), -1, dtype=torch.int64, device=DEV)
+    token[torch.where(slots >= 0, slots, pages * ps)] = torch.arange(slots.numel(), device=DEV)
+    token = token[:-1].view(pages, 1, ps, 1)
     for x, cache in ((s["k"], kc), (s["v"], vc)):
-        sel = torch.where(keep, s["slots"], kc.shape[0] * ps - 1)
-        page, at = sel // ps, sel % ps
-        cache[page, :, at] = torch.where(keep[:, None, None], x, cache[page, :, at])      # the pool's last slot takes no token of its own here
+        new = x[token.clamp(min=0).view(pages, ps)].transpose(1, 2)
+        cache.copy_(torch.where(token >= 0, new, cache))
     return [kc, vc]
 
 
