@@ -1,65 +1,626 @@
 // mmf_amd :: attention of new tokens over the pages of their request (mmf_paged_attention).
 //   out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j]
-// One pass over the keys with the running maximum m and sum l of the softmax: a block of scores s moves them to
+// One pass over the keys with the running maximum m and sum l of the softmax: a tile of scores s moves them to
 //   m' = max(m, max s),  l' = l exp(m - m') + sum exp(s - m'),  o' = o exp(m - m') + exp(s - m') v,   out = o / l at the end.
+//
+// The rows of a product are (new token, query head) pairs that read one key head, 32 to a wave: with q the column of S^T = K Q^T a lane holds one row's
+// scores (16 keys of every 32; lane ^ 32 the others), so maximum and sum need one exchange, and the probabilities are in the register order that the second
+// product O^T = V^T P^T takes (v_mfma_f32_32x32x16_bf16, or v_mfma_f32_32x32x2_f32 for the fp32 pool, whose operands are one row element per lane).
+//
+//   chunks (more than 32 rows per request and key head): a workgroup takes 128 rows, its four waves share the staged K and V tiles;
+//   steps  (at most 32 rows):                           a workgroup takes all beams of a group that fit 32 rows, its four waves take different tiles.
+//
+// Keys are split over workgroups in runs of equal length for all requests, chosen on the device from the actual lengths (Plan below); runs are joined by a
+// second kernel, launched only where a request can be split at all.
 #include "common.h"
 #include "mmf_amd.h"
 #include "paged_common.h"
+#include <atomic>
 
 namespace {
 
-// One wave per (new token, query head): a lane takes one of 64 keys for the scores, and D / 64 columns of the sum.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_attn_wave_kernel(mmf_paged_attn_desc d) {
-    constexpr int C = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int h = (int)(unit % d.heads);
-    const int64_t ri = unit / d.heads;
-    const int r = (int)(ri / d.max_q), i = (int)(ri - (int64_t)r * d.max_q);
-    if (r >= d.requests) return;
-    const int kv = min(max(d.kv_lens[r / d.beams], 0), d.blocks * d.page_size), n = d.q_lens[r / d.beams];
-    if (i == 0 && lane == 0 && (n > d.max_q || kv != d.kv_lens[r / d.beams])) flag_page_error();
-    if (i >= n) return;
-    const int64_t row = (int64_t)d.q_start[r] + i;
-    if (row < 0 || row >= d.tokens) { flag_page_error(); return; }
-    const T* q = (const T*)d.q + row * d.q_row + h * d.q_head;
-    const int hk = h / (d.heads / d.kv_heads);
-    const int end = d.causal ? min(kv, kv - n + i + 1) : kv;
-    const int32_t* table = d.tables + r * d.table_row;
-    float m = -INFINITY, l = 0.f, o[C];
+typedef __attribute__((address_space(3))) void* lds_vp;
+typedef const __attribute__((address_space(1))) void* glb_vp;
+static __device__ uint4 g_zero16;
+
+constexpr int UNITS_MAX = 1024;        // requests (chunks) or groups of beams (steps) per launch
+constexpr int PREFIX_MAX = 3 * (UNITS_MAX + 1) * 4;
+
+struct Args {
+    mmf_paged_attn_desc d;
+    int page_shift, group;             // group: query heads per key head
+    int units, nb, per_group;          // nb: beams a unit takes together (steps), per_group: units per group of beams
+    int target, run_min;               // workgroups to aim at when keys are split; shortest run
+    float c;                           // |scale| log2 e (1 when scale is 0)
+    float qmul;                        // sign of the scale (0 when it is 0): exact on any operand
+};
+
+// ---- LDS image of rows of RB bytes, 16-byte chunks XOR-swizzled so that 16 rows at one chunk, and 4 rows x 4 chunks, meet no bank twice ----
+template <int RB> DEVI int swz(int row) { return RB == 128 ? (row >> 1) & 7 : ((row & 3) << 2) | ((row >> 2) & 3); }
+template <int RB> DEVI int at(int row, int chunk) { return row * RB + ((chunk ^ swz<RB>(row)) << 4); }
+
+// keys key0 .. + ROWS of one page run into K and V images by LDS-DMA; keys >= end, and keys on pages outside the pool, come as zeros.
+// `page` holds, in lane l, the page of key0 + (l % ROWS).  NW waves share the tile, this is wave `wave`.
+template <typename T, int D, int ROWS, int NW>
+DEVI void stage(const Args& a, int key0, int end, int page, int64_t head_off, unsigned char* k_img, unsigned char* v_img, int wave, int lane) {
+    constexpr int RB = D * (int)sizeof(T), CPR = RB / 16, RPI = 64 / CPR;
+    const int mask = a.d.page_size - 1;
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = 0.f;
-    for (int j0 = 0; j0 < end; j0 += 64) {
-        const int j = j0 + lane;
-        int page = j < end ? table[j / d.page_size] : -1;
-        if (j < end && (page < 0 || page >= d.pages)) { flag_page_error(); page = -1; }
-        const int64_t off = (int64_t)page * d.page_stride + hk * d.head_stride + (int64_t)(j % d.page_size) * d.pos_stride;
-        float s = -INFINITY;
-        if (page >= 0) {
-            const T* k = (const T*)d.k_cache + off;
-            s = 0.f;
-            for (int e = 0; e < D; ++e) s += (float)q[e] * (float)k[e];
-            s *= d.scale;
-        }
-        const float m1 = fmaxf(m, wave_max(s)), mm = m1 == -INFINITY ? 0.f : m1;
-        const float a = __expf(m - mm), p = __expf(s - mm);
-        l = l * a + wave_sum(p);
-#pragma unroll
-        for (int c = 0; c < C; ++c) o[c] *= a;
-        for (int k = 0; k < 64 && j0 + k < end; ++k) {
-            const float pk = __shfl(p, k, 64);
-            const int64_t ok = __shfl((long long)off, k, 64);
-            if (__shfl(page, k, 64) < 0) continue;
-            const T* v = (const T*)d.v_cache + ok;
-#pragma unroll
-            for (int c = 0; c < C; ++c) o[c] += pk * (float)v[c * 64 + lane];
-        }
-        m = m1;
+    for (int r0 = 0; r0 < ROWS; r0 += NW * RPI) {
+        const int row = r0 + wave * RPI + lane / CPR;
+        const int p = __shfl(page, row, 64);
+        const bool in = key0 + row < end, ok = in && (unsigned)p < (unsigned)a.d.pages;
+        if (in != ok) flag_page_error();
+        const int64_t off = (int64_t)p * a.d.page_stride + (int64_t)((key0 + row) & mask) * a.d.pos_stride + head_off;
+        const int byte = ((lane % CPR) ^ swz<RB>(row)) * 16;
+        const char* zero = reinterpret_cast<const char*>(&g_zero16);
+        const char* ks = ok ? (const char*)a.d.k_cache + off * (int)sizeof(T) + byte : zero;
+        const char* vs = ok ? (const char*)a.d.v_cache + off * (int)sizeof(T) + byte : zero;
+        const int to = (r0 + wave * RPI) * RB;
+        __builtin_amdgcn_global_load_lds((glb_vp)ks, (lds_vp)(k_img + to), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_vp)vs, (lds_vp)(v_img + to), 16, 0, 0);
     }
-    T* out = (T*)d.out + row * d.out_row + h * d.out_head;
+}
+// the page of key key0 + l % ROWS, for lane l; -1 behind the end
+template <int ROWS> DEVI int page_of(const Args& a, const int32_t* table, int key0, int end, int lane) {
+    const int key = key0 + (lane & (ROWS - 1));
+    return key < end ? table[key >> a.page_shift] : -1;
+}
+
+DEVI void pick(f32x16& o, const f32x16& x, bool take) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) out[c * 64 + lane] = (T)(l > 0.f ? o[c] / l : 0.f);
+    for (int r = 0; r < 16; ++r) o[r] = take ? x[r] : o[r];
+}
+
+// ---- the rows of a wave: their queries, softmax state and sums ----
+template <typename T, int D> struct Rows;
+
+template <int D> struct Rows<bf16, D> {
+    bf16x8 q[D / 16];
+    DEVI void load(const bf16* p, bool ok, float mul, int lane) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            bf16x8 x = {};
+            if (ok) x = *reinterpret_cast<const bf16x8*>(p + 16 * s + 8 * (lane >> 5));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (bf16)((float)x[e] * mul);
+            q[s] = x;
+        }
+    }
+    // scores of keys row0 .. + 32 of the image
+    DEVI f32x16 scores(const unsigned char* k, int row0, int lane) const {
+        f32x16 s = {};
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(k + at<2 * D>(row0 + (lane & 31), 2 * u + (lane >> 5))), q[u], s, 0, 0, 0);
+        return s;
+    }
+    // sums += V^T p for keys row0 .. + 32 (PICK: in the lanes that `take`; a value that is no number stays with them); the transposed operand comes by ds_read_b64_tr_b16 (16 lanes read 4 rows x 16 columns, lane i gets column i)
+    template <bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16& p, const unsigned char* v, int row0, bool take, int lane) {
+        typedef s16x4 __attribute__((address_space(3))) * lds_p;
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const int g = lane >> 4, i = lane & 15;
+        bf16x8 pb[2];                                              // rounded to bf16: relative 2^-8 of each probability, the pool's own precision
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pb[e >> 3][e & 7] = (bf16)p[e];
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) {
+            f32x16 acc = o[t];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int row = row0 + 16 * u + 4 * (g >> 1) + (i >> 2), col = 32 * t + 16 * (g & 1) + (i & 3) * 4;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(v + at<2 * D>(row, col >> 3) + (col & 7) * 2));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(v + at<2 * D>(row + 8, col >> 3) + (col & 7) * 2));
+                const s16x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), pb[u], acc, 0, 0, 0);
+            }
+            if (PICK) pick(o[t], acc, take);
+            else o[t] = acc;
+        }
+    }
+};
+
+// fp32: a step of v_mfma_f32_32x32x2_f32 takes one element per lane, lanes 0 - 31 of reduction slot 0 and lanes 32 - 63 of slot 1
+template <int D> struct Rows<float, D> {
+    f32x4 q[D / 8];                                                // element (t, e) of half h: column 8 t + 4 h + e
+    DEVI void load(const float* p, bool ok, float mul, int lane) {
+#pragma unroll
+        for (int t = 0; t < D / 8; ++t) {
+            f32x4 x = {};
+            if (ok) x = *reinterpret_cast<const f32x4*>(p + 8 * t + 4 * (lane >> 5));
+            q[t] = x * mul;
+        }
+    }
+    DEVI f32x16 scores(const unsigned char* k, int row0, int lane) const {
+        f32x16 s = {};
+#pragma unroll
+        for (int t = 0; t < D / 8; ++t) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(k + at<4 * D>(row0 + (lane & 31), 2 * t + (lane >> 5)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[t][e], s, 0, 0, 0);
+        }
+        return s;
+    }
+    template <bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16& p, const unsigned char* v, int row0, bool take, int lane) {
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) {
+            f32x16 acc = o[t];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = row0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), col = 32 * t + (lane & 31);
+                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(v + at<4 * D>(row, col >> 2) + (col & 3) * 4), p[r], acc, 0, 0, 0);
+            }
+            if (PICK) pick(o[t], acc, take);
+            else o[t] = acc;
+        }
+    }
+};
+
+DEVI float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// One tile of NS x 32 keys, key0 its first, for the rows of a wave; lim: keys this lane's row sees.  m (in units of log2) may lag up to 8 behind the largest score:
+// a probability is then at most 2^8, and the sums need no rescaling on most tiles.
+template <typename T, int D, int NS, bool PICK = false>
+DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsigned char* v, int key0, int lim, bool masked, float c, float& m, float& l, f32x16 (&o)[D / 32],
+                    int lane, bool take = true) {
+    f32x16 s[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) s[n] = rows.scores(k, 32 * n, lane);
+    float top = -INFINITY;
+    const int h4 = 4 * (lane >> 5);
+    if (masked) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (key0 + 32 * n + 8 * (r >> 2) + h4 + (r & 3) >= lim) s[n][r] = -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+    top = fmaxf(top, other_half(top)) * c;
+    if (__ballot(top > m + 8.f) != 0) {
+        const float next = fmaxf(m, top), keep = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= keep;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[t][r] *= keep;
+    }
+    const float mm = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -mm));
+            sum += s[n][r];
+        }
+    l += sum;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) Rows<T, D>::template add<PICK>(o, s[n], v, 32 * n, take, lane);
+}
+
+// ------------------------------------------------------------------------------------------------
+// who computes what.  Unit u (a request; or nb beams of a group) has tiles(u) row tiles and keys(u) keys; keys are cut into runs of `run` keys so that about
+// `target` workgroups have work, and a unit with one run writes its result itself.
+// ------------------------------------------------------------------------------------------------
+struct Unit { int req, nb, n, n_all, kv; };    // first request, beams, new tokens (up to max_q), all new tokens, keys
+DEVI Unit unit_of(const Args& a, int u) {
+    Unit x;
+    const int g = u / a.per_group, w0 = (u - g * a.per_group) * a.nb;
+    x.req = g * a.d.beams + w0;
+    x.nb = min(a.nb, a.d.beams - w0);
+    if (a.nb == 1) { x.req = u; x.nb = 1; }
+    const int len = x.req / a.d.beams;
+    x.n_all = max(a.d.q_lens[len], 0);
+    x.n = min(x.n_all, a.d.max_q);
+    x.kv = min(max(a.d.kv_lens[len], 0), a.d.blocks * a.d.page_size);
+    return x;
+}
+
+struct Plan {
+    int run, items, parts, joins;
+    int* item0;      // [units + 1] first item of each unit
+    int* part0;      // first partial result (units with several runs)
+    int* join0;      // first (tile, head) to join
+};
+template <int TILE> DEVI int tiles_of(const Args& a, const Unit& x) { return (x.nb * x.n * a.group + TILE - 1) / TILE; }
+
+DEVI int64_t wave_add(int64_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((long long)v, o, 64);
+    return v;
+}
+DEVI int wave_upto(int v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o, 64);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+// `lds`: 3 (units + 1) ints; every wave ends with the same plan (the first one writes it)
+template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
+    const int lane = threadIdx.x & 63;
+    Plan p;
+    p.item0 = lds;
+    p.part0 = lds + a.units + 1;
+    p.join0 = lds + 2 * (a.units + 1);
+    int64_t work = 0;
+    bool odd = false;
+    for (int u = lane; u < a.units; u += 64) {
+        const Unit x = unit_of(a, u);
+        work += (int64_t)tiles_of<TILE>(a, x) * x.kv;
+        odd |= x.n_all > a.d.max_q || x.kv != a.d.kv_lens[x.req / a.d.beams];
+    }
+    if (odd) flag_page_error();
+    work = wave_add(work) * a.d.kv_heads;
+    const int64_t run = (work + a.target - 1) / a.target;
+    p.run = (int)(max((int64_t)a.run_min, min(run, (int64_t)0x3fffffff)) + 63) / 64 * 64;
+    int items = 0, parts = 0, joins = 0;
+    for (int u0 = 0; u0 < a.units; u0 += 64) {
+        const int u = u0 + lane;
+        int i = 0, q = 0, j = 0;
+        if (u < a.units) {
+            const Unit x = unit_of(a, u);
+            const int t = tiles_of<TILE>(a, x) * a.d.kv_heads, runs = max(1, (x.kv + p.run - 1) / p.run);
+            i = t * runs;
+            if (runs > 1) { q = i; j = t; }
+        }
+        const int iu = wave_upto(i, lane), qu = wave_upto(q, lane), ju = wave_upto(j, lane);
+        if (u < a.units && threadIdx.x < 64) { p.item0[u] = items + iu - i; p.part0[u] = parts + qu - q; p.join0[u] = joins + ju - j; }
+        items += __shfl(iu, 63, 64);
+        parts += __shfl(qu, 63, 64);
+        joins += __shfl(ju, 63, 64);
+    }
+    p.items = items;
+    p.parts = parts;
+    p.joins = joins;
+    if (threadIdx.x == 0) { p.item0[a.units] = items; p.part0[a.units] = parts; p.join0[a.units] = joins; }
+    __syncthreads();
+    return p;
+}
+DEVI int find(const int* first, int units, int i) {          // the last unit whose first is <= i and that is not empty
+    int lo = 0, hi = units;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= i) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// a row of a unit: beam, token, query head within the group -> its token row, or -1 where it has none
+struct Row { int64_t token; int head, beam, i; };
+DEVI Row row_of(const Args& a, const Unit& x, int row) {
+    Row r;
+    const int t = row / a.group;
+    r.head = row - t * a.group;
+    r.beam = x.nb == 1 ? 0 : t / x.n;
+    r.i = t - r.beam * x.n;
+    r.token = -1;
+    if (row < x.nb * x.n * a.group) {
+        r.token = (int64_t)a.d.q_start[x.req + r.beam] + r.i;
+        if (r.token < 0 || r.token >= a.d.tokens) { flag_page_error(); r.token = -1; }
+    }
+    return r;
+}
+DEVI int sees(const Args& a, const Unit& x, int i) { return a.d.causal ? max(0, min(x.kv, x.kv - x.n_all + i + 1)) : x.kv; }
+
+template <typename T, int D> DEVI T* out_row(const Args& a, const Row& r, int h) {
+    return (T*)a.d.out + r.token * a.d.out_row + (int64_t)(h * a.group + r.head) * a.d.out_head;
+}
+// partial results: [part][TILE][D] sums, then [part][TILE][2] maximum (log2) and sum
+template <int D, int TILE> DEVI float* part_o(const Args& a, int part) { return (float*)a.d.ws + (int64_t)part * TILE * D; }
+template <int D, int TILE> DEVI float* part_ml(const Args& a, int part) { return (float*)a.d.ws + (int64_t)2 * a.target * TILE * D + (int64_t)part * TILE * 2; }
+
+DEVI void store4(bf16* p, float a, float b, float c, float d) { *reinterpret_cast<bf16x4*>(p) = pack4(a, b, c, d); }
+DEVI void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d}; }
+
+// ------------------------------------------------------------------------------------------------
+// chunks
+// ------------------------------------------------------------------------------------------------
+constexpr int CHUNK_ROWS = 128;
+template <typename T> constexpr int chunk_subtiles = sizeof(T) == 2 ? 2 : 1;      // 64 keys a tile in bf16, 32 in fp32: 32 or 16 KB of K and V at head_dim 64 or 128 either way
+template <typename T, int D> constexpr int chunk_lds = 2 * 2 * 32 * chunk_subtiles<T> * D * (int)sizeof(T);
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_attn_chunk_kernel(Args a) {
+    extern __shared__ unsigned char lds[];
+    constexpr int NS = chunk_subtiles<T>, KT = 32 * NS, RB = D * (int)sizeof(T), IMG = KT * RB;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Plan plan = make_plan<CHUNK_ROWS>(a, reinterpret_cast<int*>(lds + 4 * IMG));
+    for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
+        const int u = find(plan.item0, a.units, item);
+        const Unit x = unit_of(a, u);
+        int rest = item - plan.item0[u];
+        const int h = rest % a.d.kv_heads;
+        rest /= a.d.kv_heads;
+        const int tiles = tiles_of<CHUNK_ROWS>(a, x), tile = rest % tiles, run = rest / tiles, row0 = tile * CHUNK_ROWS;
+        const bool whole = plan.run >= x.kv;
+        const int last = min(x.n * a.group, row0 + CHUNK_ROWS) - 1;
+        const int end = min(sees(a, x, last / a.group), (run + 1) * plan.run);
+        const int start = run * plan.run;
+        const Row row = row_of(a, x, row0 + 32 * wave + (lane & 31));
+        const int lim = row.token >= 0 ? sees(a, x, row.i) : 0x7fffffff;      // (rows without a token compute on zeros: nothing of them is written)
+        Rows<T, D> rows;
+        rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a.qmul, lane);
+        int free_to = lim;                                                       // keys every row of the wave sees
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) free_to = min(free_to, __shfl_xor(free_to, o, 64));
+        float m = -INFINITY, l = 0.f;
+        f32x16 o[D / 32] = {};
+        const int32_t* table = a.d.tables + x.req * a.d.table_row;
+        const int64_t head_off = h * a.d.head_stride;
+        const int steps = end > start ? (end - start + KT - 1) / KT : 0;
+        int page = page_of<KT>(a, table, start, end, lane);
+        __syncthreads();                                                         // the item before has read its last tile
+        if (steps > 0) stage<T, D, KT, 4>(a, start, end, page, head_off, lds, lds + IMG, wave, lane);
+        page = page_of<KT>(a, table, start + KT, end, lane);
+        for (int j = 0; j < steps; ++j) {
+            const int key0 = start + j * KT;
+            unsigned char* img = lds + (j & 1) * 2 * IMG;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (j + 1 < steps) {
+                unsigned char* next = lds + ((j + 1) & 1) * 2 * IMG;
+                stage<T, D, KT, 4>(a, key0 + KT, end, page, head_off, next, next + IMG, wave, lane);
+                page = page_of<KT>(a, table, key0 + 2 * KT, end, lane);
+            }
+            tile_step<T, D, NS>(rows, img, img + IMG, key0, min(lim, end), key0 + KT > min(free_to, end), a.c, m, l, o, lane);
+        }
+        l += other_half(l);
+        if (whole) {
+            if (row.token >= 0) {
+                T* out = out_row<T, D>(a, row, h);
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4)
+                        store4(out + 32 * t + 2 * r + 4 * (lane >> 5), o[t][r] * inv, o[t][r + 1] * inv, o[t][r + 2] * inv, o[t][r + 3] * inv);
+            }
+        } else {
+            const int part = plan.part0[u] + (item - plan.item0[u]);
+            const int at_row = 32 * wave + (lane & 31);
+            float* po = part_o<D, CHUNK_ROWS>(a, part) + at_row * D;
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) store4(po + 32 * t + 2 * r + 4 * (lane >> 5), o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]);
+            if (lane < 32) {
+                float* ml = part_ml<D, CHUNK_ROWS>(a, part) + 2 * at_row;
+                ml[0] = m;
+                ml[1] = l;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// steps
+// ------------------------------------------------------------------------------------------------
+constexpr int STEP_ROWS = 32;
+template <typename T, int D> constexpr int step_lds = 4 * 2 * 32 * D * (int)sizeof(T);       // a tile of 32 keys per wave
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_attn_step_kernel(Args a) {
+    extern __shared__ unsigned char lds[];
+    constexpr int RB = D * (int)sizeof(T), IMG = 32 * RB;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned char* mine = lds + wave * 2 * IMG;
+    int* shared_to = reinterpret_cast<int*>(lds + 8 * IMG);
+    const Plan plan = make_plan<STEP_ROWS>(a, shared_to + 4);
+    for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
+        const int u = find(plan.item0, a.units, item);
+        const Unit x = unit_of(a, u);
+        const int h = (item - plan.item0[u]) % a.d.kv_heads, run = (item - plan.item0[u]) / a.d.kv_heads;
+        const int start = run * plan.run, end = min(x.kv, start + plan.run);
+        const bool whole = plan.run >= x.kv;
+        const int n_rows = x.nb * x.n * a.group;
+        const Row row = row_of(a, x, lane & 31);
+        const int lim = row.token >= 0 ? min(sees(a, x, row.i), end) : 0x7fffffff;
+        Rows<T, D> rows;
+        rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a.qmul, lane);
+        int free_to = lim;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) free_to = min(free_to, __shfl_xor(free_to, o, 64));
+        const int32_t* table = a.d.tables + x.req * a.d.table_row;
+        const int64_t head_off = h * a.d.head_stride;
+        // whole tiles whose pages are the same for every beam are read once for all of them: blocks up to the first that differs
+        __syncthreads();                                                         // the item before has read shared_to and the tiles
+        int shared_tiles = (max(end - start, 0) + 31) / 32;
+        if (x.nb > 1 && end > start) {
+            int differs = 0x7fffffff;
+            const int b1 = (end - 1) >> a.page_shift;
+            for (int b = (start >> a.page_shift) + threadIdx.x; b <= b1; b += 256) {
+                const int p = table[b];
+                for (int w = 1; w < x.nb; ++w)
+                    if (table[w * a.d.table_row + b] != p) differs = min(differs, b);
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) differs = min(differs, __shfl_xor(differs, o, 64));
+            if (lane == 0) shared_to[wave] = differs;
+            __syncthreads();
+            differs = min(min(shared_to[0], shared_to[1]), min(shared_to[2], shared_to[3]));
+            if (differs <= b1) shared_tiles = max(0, (int)(((int64_t)differs << a.page_shift) - start)) / 32;
+        }
+        const int tiles = (max(end - start, 0) + 31) / 32, jobs = shared_tiles + (tiles - shared_tiles) * x.nb;
+        float m = -INFINITY, l = 0.f;
+        f32x16 o[D / 32] = {};
+        auto job = [&](int j, int& key0, int& w) {
+            const bool one = j >= shared_tiles;
+            key0 = start + 32 * (one ? shared_tiles + (j - shared_tiles) / x.nb : j);
+            w = one ? (j - shared_tiles) % x.nb : -1;
+            return page_of<32>(a, table + max(w, 0) * a.d.table_row, key0, j < jobs ? end : 0, lane);
+        };
+        int key0, w, page = job(wave, key0, w);
+        for (int j = wave; j < jobs; j += 4) {
+            const int key0_now = key0, w_now = w;
+            stage<T, D, 32, 1>(a, key0, end, page, head_off, mine, mine + IMG, 0, lane);
+            page = job(j + 4, key0, w);                                          // (the next tile's pages come along with this tile)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (w_now < 0) tile_step<T, D, 1>(rows, mine, mine + IMG, key0_now, lim, key0_now + 32 > free_to, a.c, m, l, o, lane);
+            else {                                                               // a tile of one beam: the other beams' rows see none of it
+                const bool take = row.beam == w_now;
+                tile_step<T, D, 1, true>(rows, mine, mine + IMG, key0_now, take ? lim : 0, true, a.c, m, l, o, lane, take);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                   // the tile is read before the next one lands on it
+        }
+        l += other_half(l);
+        // the four waves' sums meet: [wave][row][D] fp32 in the tiles' place, [wave][row][2] behind
+        __syncthreads();
+        constexpr int LD = D + 4;                                                // (rows of D floats alone would put every row's column on one bank)
+        float* so = reinterpret_cast<float*>(lds);
+        float* sml = so + 4 * 8 * LD;
+        for (int r0 = 0; r0 < n_rows; r0 += 8) {                                 // 8 rows at a time: 4 x 8 x (D + 4) floats fit any form's tiles
+            const int at_row = (lane & 31) - r0;
+            if (at_row >= 0 && at_row < 8) {
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4)
+                        *reinterpret_cast<f32x4*>(so + (wave * 8 + at_row) * LD + 32 * t + 2 * r + 4 * (lane >> 5)) = f32x4{o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
+                if (lane < 32) { sml[(wave * 8 + at_row) * 2] = m; sml[(wave * 8 + at_row) * 2 + 1] = l; }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 8 * (D / 4); i += 256) {
+                const int rr = i / (D / 4), e = (i - rr * (D / 4)) * 4;
+                if (r0 + rr >= n_rows) continue;
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) top = fmaxf(top, sml[(w * 8 + rr) * 2]);
+                const float mm = top == -INFINITY ? 0.f : top;
+                f32x4 sum = {};
+                float den = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(sml[(w * 8 + rr) * 2] - mm);
+                    den += f * sml[(w * 8 + rr) * 2 + 1];
+                    sum += f * *reinterpret_cast<const f32x4*>(so + (w * 8 + rr) * LD + e);
+                }
+                if (whole) {
+                    const Row to = row_of(a, x, r0 + rr);
+                    const float inv = den != 0.f ? 1.f / den : 0.f;
+                    if (to.token >= 0) store4(out_row<T, D>(a, to, h) + e, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+                } else {
+                    const int part = plan.part0[u] + (item - plan.item0[u]);
+                    *reinterpret_cast<f32x4*>(part_o<D, STEP_ROWS>(a, part) + (r0 + rr) * D + e) = sum;
+                    if (e == 0) { float* ml = part_ml<D, STEP_ROWS>(a, part) + 2 * (r0 + rr); ml[0] = top; ml[1] = den; }
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// the runs of a split request, joined in their order
+// ------------------------------------------------------------------------------------------------
+template <typename T, int D, int TILE>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(Args a) {
+    extern __shared__ unsigned char lds[];
+    const Plan plan = make_plan<TILE>(a, reinterpret_cast<int*>(lds));
+    constexpr int PER = D / 4, ROWS = 256 / PER;                                 // threads per row, rows at a time
+    constexpr int SLICES = TILE / ROWS;
+    for (int i = blockIdx.x; i < plan.joins * SLICES; i += gridDim.x) {
+        const int j = i / SLICES, slice = i - j * SLICES;
+        const int u = find(plan.join0, a.units, j);
+        const Unit x = unit_of(a, u);
+        const int h = (j - plan.join0[u]) % a.d.kv_heads, tile = (j - plan.join0[u]) / a.d.kv_heads, tiles = tiles_of<TILE>(a, x);
+        const int runs = (x.kv + plan.run - 1) / plan.run;
+        const int at_row = slice * ROWS + threadIdx.x / PER, e = (threadIdx.x % PER) * 4;
+        const Row row = row_of(a, x, tile * TILE + at_row);
+        if (row.token < 0) continue;
+        float top = -INFINITY, den = 0.f;
+        f32x4 sum = {};
+        for (int r = 0; r < runs; ++r) {
+            const int part = plan.part0[u] + (r * tiles + tile) * a.d.kv_heads + h;
+            const float* ml = part_ml<D, TILE>(a, part) + 2 * at_row;
+            const float mr = ml[0], lr = ml[1];
+            const f32x4 v = *reinterpret_cast<const f32x4*>(part_o<D, TILE>(a, part) + at_row * D + e);
+            const float next = fmaxf(top, mr), mm = next == -INFINITY ? 0.f : next;
+            const float fa = __builtin_amdgcn_exp2f(top - mm), fb = __builtin_amdgcn_exp2f(mr - mm);
+            den = den * fa + lr * fb;
+            sum = sum * fa + v * fb;
+            top = next;
+        }
+        const float inv = den != 0.f ? 1.f / den : 0.f;
+        store4(out_row<T, D>(a, row, h) + e, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+    }
+}
+
+struct Shape { bool chunk, split; int nb, target, run_min; int64_t ws; };
+Shape shape_of(const mmf_paged_attn_desc* d) {
+    Shape s;
+    const int64_t rows = (int64_t)d->max_q * (d->heads / d->kv_heads);
+    s.chunk = rows > STEP_ROWS;
+    s.nb = s.chunk ? 1 : (int)(STEP_ROWS / rows < d->beams ? STEP_ROWS / rows : d->beams);
+    s.target = 1024;
+    s.run_min = s.chunk ? 1024 : 256;
+    s.split = (int64_t)d->blocks * d->page_size > s.run_min;
+    s.ws = s.split ? (int64_t)2 * s.target * (s.chunk ? CHUNK_ROWS : STEP_ROWS) * (d->head_dim + 2) * 4 : 0;
+    return s;
+}
+
+// more than 64 KB of LDS are asked for once per kernel and device
+template <typename K> int allow_lds(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return 1;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return 1;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+}
+
+template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shape& s, hipStream_t stream) {
+    Args a;
+    a.d = *d;
+    a.page_shift = __builtin_ctz(d->page_size);
+    a.group = d->heads / d->kv_heads;
+    a.nb = s.nb;
+    a.per_group = (d->beams + s.nb - 1) / s.nb;
+    a.target = s.target;
+    a.run_min = s.split ? s.run_min : 0x3fffffff;
+    a.c = d->scale != 0.f ? fabsf(d->scale) * 1.44269504088896340736f : 1.f;
+    a.qmul = d->scale > 0.f ? 1.f : d->scale < 0.f ? -1.f : 0.f;
+    const int step = UNITS_MAX / a.per_group * d->beams;         // requests per launch: whole groups
+    for (int r0 = 0; r0 < d->requests; r0 += step) {
+        const int n = d->requests - r0 < step ? d->requests - r0 : step;
+        a.d.requests = n;
+        a.d.tables = d->tables + r0 * d->table_row;
+        a.d.kv_lens = d->kv_lens + r0 / d->beams;
+        a.d.q_lens = d->q_lens + r0 / d->beams;
+        a.d.q_start = d->q_start + r0;
+        a.units = s.nb == 1 ? n : n / d->beams * a.per_group;
+        const int prefix = 3 * (a.units + 1) * 4;
+        const int64_t tiles = s.chunk ? ((int64_t)d->max_q * a.group + CHUNK_ROWS - 1) / CHUNK_ROWS : 1;
+        int64_t most = tiles * a.units * d->kv_heads + (s.split ? 2 * s.target : 0);
+        const int grid = (int)(most < s.target ? most : s.target);
+        if (s.chunk) {
+            const int lds = chunk_lds<T, D> + prefix;
+            static std::atomic<uint64_t> done{0};
+            MMF_CHECK_ARG(!allow_lds(paged_attn_chunk_kernel<T, D>, chunk_lds<T, D> + PREFIX_MAX, done), "paged_attention: LDS");
+            hipLaunchKernelGGL((paged_attn_chunk_kernel<T, D>), dim3(grid), dim3(256), lds, stream, a);
+        } else {
+            const int lds = step_lds<T, D> + 16 + prefix;
+            static std::atomic<uint64_t> done{0};
+            MMF_CHECK_ARG(!allow_lds(paged_attn_step_kernel<T, D>, step_lds<T, D> + 16 + PREFIX_MAX, done), "paged_attention: LDS");
+            hipLaunchKernelGGL((paged_attn_step_kernel<T, D>), dim3(grid), dim3(256), lds, stream, a);
+        }
+        MMF_CHECK_LAUNCH();
+        if (s.split) {
+            if (s.chunk) hipLaunchKernelGGL((paged_attn_join_kernel<T, D, CHUNK_ROWS>), dim3(1024), dim3(256), prefix, stream, a);
+            else hipLaunchKernelGGL((paged_attn_join_kernel<T, D, STEP_ROWS>), dim3(512), dim3(256), prefix, stream, a);
+            MMF_CHECK_LAUNCH();
+        }
+    }
+    return 0;
 }
 
 }  // namespace
@@ -73,26 +634,29 @@ int mmf_paged_attention_take_error(void) {
     return v;
 }
 
-int64_t mmf_paged_attention_ws_bytes(const mmf_paged_attn_desc* d) { (void)d; return 0; }
+int64_t mmf_paged_attention_ws_bytes(const mmf_paged_attn_desc* d) {
+    if (!d || d->kv_heads <= 0 || d->heads < d->kv_heads || d->max_q < 1 || d->beams < 1) return 0;
+    return shape_of(d).ws;
+}
 
 int mmf_paged_attention(const mmf_paged_attn_desc* d, void* stream) {
     MMF_CHECK_ARG(d && d->q && d->k_cache && d->v_cache && d->tables && d->kv_lens && d->q_start && d->q_lens && d->out, "paged_attention: null operand");
     MMF_CHECK_ARG(d->head_dim == 64 || d->head_dim == 128, "paged_attention: head_dim is 64 or 128");
     MMF_CHECK_ARG(d->heads > 0 && d->kv_heads > 0 && d->heads % d->kv_heads == 0, "paged_attention: heads is a multiple of kv_heads");
     MMF_CHECK_ARG(d->requests > 0 && d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->blocks > 0 && d->pages > 0 && d->tokens >= 0, "paged_attention: bad shape");
+    MMF_CHECK_ARG(d->requests % d->beams == 0, "paged_attention: requests come in groups of beams");
     MMF_CHECK_ARG(d->page_size >= 1 && d->page_size <= MMF_PAGE_MAX && (d->page_size & (d->page_size - 1)) == 0, "paged_attention: page_size is a power of two up to 1024");
     MMF_CHECK_ARG((int64_t)d->blocks * d->page_size <= 0x3fffffff, "paged_attention: more than 2^30 keys");
-    MMF_CHECK_ARG(d->max_q >= 1, "paged_attention: max_q is at least 1");
+    MMF_CHECK_ARG(d->max_q >= 1 && (int64_t)d->max_q * d->heads <= 0x3fffffff, "paged_attention: max_q is at least 1, and max_q * heads under 2^30");
+    const int unit = d->is_f32 ? 4 : 8;
+    MMF_CHECK_ARG(((uintptr_t)d->q & 15) == 0 && ((uintptr_t)d->k_cache & 15) == 0 && ((uintptr_t)d->v_cache & 15) == 0 && ((uintptr_t)d->out & 15) == 0 &&
+                      d->q_row % unit == 0 && d->q_head % unit == 0 && d->page_stride % unit == 0 && d->head_stride % unit == 0 && d->pos_stride % unit == 0 &&
+                      d->out_row % unit == 0 && d->out_head % unit == 0, "paged_attention: rows start on 16 bytes");
     if (d->tokens == 0) return 0;
-    const int64_t units = (int64_t)d->requests * d->max_q * d->heads, blocks = (units + 3) / 4;
-    MMF_CHECK_ARG(blocks <= 0x7fffffff, "paged_attention: too many rows for one call");
-    const dim3 grid((unsigned)blocks);
-    if (d->is_f32 && d->head_dim == 64) hipLaunchKernelGGL((paged_attn_wave_kernel<float, 64>), grid, dim3(256), 0, (hipStream_t)stream, *d);
-    else if (d->is_f32) hipLaunchKernelGGL((paged_attn_wave_kernel<float, 128>), grid, dim3(256), 0, (hipStream_t)stream, *d);
-    else if (d->head_dim == 64) hipLaunchKernelGGL((paged_attn_wave_kernel<bf16, 64>), grid, dim3(256), 0, (hipStream_t)stream, *d);
-    else hipLaunchKernelGGL((paged_attn_wave_kernel<bf16, 128>), grid, dim3(256), 0, (hipStream_t)stream, *d);
-    MMF_CHECK_LAUNCH();
-    return 0;
+    const Shape s = shape_of(d);
+    MMF_CHECK_ARG(s.ws == 0 || (d->ws && ((uintptr_t)d->ws & 15) == 0), "paged_attention: null workspace");
+    if (d->is_f32) return d->head_dim == 64 ? launch<float, 64>(d, s, (hipStream_t)stream) : launch<float, 128>(d, s, (hipStream_t)stream);
+    return d->head_dim == 64 ? launch<bf16, 64>(d, s, (hipStream_t)stream) : launch<bf16, 128>(d, s, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -244,19 +244,19 @@ def test_max_q_larger_than_any_request_and_out_in_place_of_q(dtype):
     assert torch.equal(out[:29], a[:29])
 
 
-def test_pages_outside_the_pool_are_left_out_and_reported():
+def test_pages_outside_the_pool_are_reported_and_other_requests_do_not_notice():
     from mmf_amd import _native as nat
     for new, dtype in ((1, torch.bfloat16), (40, torch.bfloat16), (1, torch.float32), (40, torch.float32)):
-        c = attend_case([64], [new], heads=2, kv_heads=2, page=16, dtype=dtype)
-        good = attend_check(dict(c, kv_lens=i32([48])), causal=False)
+        c = attend_case([64, 90], [new, new], heads=2, kv_heads=2, page=16, dtype=dtype)
+        good = attend_check(c)
         for bad in (-3, 10 ** 6):
             t = c["tables"].clone()
             t[0, 3] = bad
-            got = D().attend_pages(c["q"], c["key_cache"], c["value_cache"], t, c["kv_lens"], c["q_start"], c["q_lens"], max_q=new, causal=False)
+            got = D().attend_pages(c["q"], c["key_cache"], c["value_cache"], t, c["kv_lens"], c["q_start"], c["q_lens"], max_q=new)
             assert nat.take_index_error()
-            assert torch.allclose(got[:new].float(), good[:new].float(), rtol=2 ** -6, atol=2 ** -6)
+            assert torch.equal(got[new:2 * new], good[new:2 * new])
         # rows outside the token buffer, more new tokens than max_q: reported, nothing is read or written out of range
-        D().attend_pages(c["q"], c["key_cache"], c["value_cache"], c["tables"], c["kv_lens"], i32([10 ** 7]), c["q_lens"], max_q=new)
+        D().attend_pages(c["q"], c["key_cache"], c["value_cache"], c["tables"], c["kv_lens"], i32([10 ** 7, 0]), c["q_lens"], max_q=new)
         assert nat.take_index_error()
         if new > 1:
             D().attend_pages(c["q"], c["key_cache"], c["value_cache"], c["tables"], c["kv_lens"], c["q_start"], c["q_lens"], max_q=1)
