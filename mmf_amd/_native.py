@@ -1248,111 +1248,3 @@ def probe_mfma32(a, b, d):
 
 def probe_tr16(img, addr, out):
     _check(lib().mmf_probe_tr16(_p(img), _p(addr), _p(out), _stream()), "mmf_probe_tr16")
-
-
-# --------------------------------------------------------------------------------------------
-# decoding with a paged key / value cache and beams (mmf_amd/decoding.py checks the arguments)
-# --------------------------------------------------------------------------------------------
-BEAMS_MAX, PAGE_MAX = 32, 1024
-
-
-class PagedPlanDesc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("q_lens", "kv_lens", "tables", "owned", "free_pages", "free_top", "q_start", "granted", "kv_out", "slots", "positions",
-                                          "copies", "top_out", "refused", "ws")] + \
-               [(n, C.c_int) for n in ("groups", "beams", "blocks", "page_size", "rows", "shared", "free_capacity")]
-
-
-class PagedWriteDesc(C.Structure):
-    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in ("k_row", "k_head", "v_row", "v_head")] + \
-               [("k_cache", C.c_void_p), ("v_cache", C.c_void_p)] + [(n, C.c_int64) for n in ("page_stride", "head_stride", "pos_stride")] + \
-               [("slots", C.c_void_p)] + [(n, C.c_int) for n in ("tokens", "pages", "page_size", "kv_heads", "head_dim", "is_f32")]
-
-
-class PagedAttnDesc(C.Structure):
-    _fields_ = [("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p)] + \
-               [(n, C.c_int64) for n in ("page_stride", "head_stride", "pos_stride")] + [("tables", C.c_void_p), ("table_row", C.c_int64)] + \
-               [(n, C.c_void_p) for n in ("kv_lens", "q_start", "q_lens", "out")] + [("out_row", C.c_int64), ("out_head", C.c_int64), ("ws", C.c_void_p)] + \
-               [(n, C.c_int) for n in ("tokens", "requests", "beams", "blocks", "pages", "page_size", "heads", "kv_heads", "head_dim", "max_q", "causal", "is_f32")] + \
-               [("scale", C.c_float)]
-
-
-class BeamSelectDesc(C.Structure):
-    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64)] + \
-               [(n, C.c_void_p) for n in ("scores", "finished", "history", "scores_out", "parents", "tokens", "finished_out", "history_out", "ws")] + \
-               [(n, C.c_int64) for n in ("vocab", "eos", "length", "step")] + [(n, C.c_int) for n in ("groups", "beams", "is_f32")]
-
-
-class PagedReorderDesc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("parents", "kv_lens", "tables", "tables_out", "copies")] + [(n, C.c_int) for n in ("groups", "beams", "blocks", "page_size")]
-
-
-class PagedCopyDesc(C.Structure):
-    _fields_ = [("copies", C.c_void_p), ("cache", C.c_void_p)] + [(n, C.c_int64) for n in ("plane_stride", "page_stride", "head_stride", "pos_stride")] + \
-               [(n, C.c_int) for n in ("rows", "planes", "pages", "page_size", "kv_heads", "head_dim", "is_f32")]
-
-
-def _a(t):
-    """Device address of a tensor for a descriptor field (or None)."""
-    return None if t is None else t.data_ptr()
-
-
-def _ws(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def paged_plan(q_lens, kv_lens, tables, owned, free_pages, free_top, q_start, granted, kv_out, slots, positions, copies, top_out, refused, beams, page_size,
-               shared):
-    f = lib().mmf_paged_plan_ws_bytes
-    f.restype = C.c_int64
-    groups = q_lens.numel()
-    ws = _ws(f(groups), q_lens.device)
-    d = PagedPlanDesc(_a(q_lens), _a(kv_lens), _a(tables), _a(owned), _a(free_pages), _a(free_top), _a(q_start), _a(granted), _a(kv_out), _a(slots), _a(positions),
-                      _a(copies), _a(top_out), _a(refused), _a(ws), groups, beams, tables.shape[1], page_size, slots.numel(), int(shared), free_pages.numel())
-    _check(lib().mmf_paged_plan(C.byref(d), _stream()), "mmf_paged_plan")
-
-
-def paged_write(k, v, k_cache, v_cache, slots):
-    pages, heads, page_size, dim = k_cache.shape
-    d = PagedWriteDesc(_a(k), _a(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _a(k_cache), _a(v_cache), k_cache.stride(0), k_cache.stride(1),
-                       k_cache.stride(2), _a(slots), slots.numel(), pages, page_size, heads, dim, int(k.dtype == torch.float32))
-    _check(lib().mmf_paged_write(C.byref(d), _stream()), "mmf_paged_write")
-
-
-def paged_attention(q, k_cache, v_cache, tables, kv_lens, q_start, q_lens, out, beams, max_q, causal, scale):
-    pages, kv_heads, page_size, dim = k_cache.shape
-    d = PagedAttnDesc(_a(q), q.stride(0), q.stride(1), _a(k_cache), _a(v_cache), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), _a(tables),
-                      tables.stride(0), _a(kv_lens), _a(q_start), _a(q_lens), _a(out), out.stride(0), out.stride(1), None, q.shape[0], tables.shape[0], beams,
-                      tables.shape[1], pages, page_size, q.shape[1], kv_heads, dim, max_q, int(causal), int(q.dtype == torch.float32), scale)
-    L = lib()
-    f = L.mmf_paged_attention_ws_bytes
-    f.restype = C.c_int64
-    ws = _ws(f(C.byref(d)), q.device)
-    d.ws = _a(ws)
-    _check(L.mmf_paged_attention(C.byref(d), _stream()), "mmf_paged_attention")
-
-
-def beam_select(logits, scores, finished, history, scores_out, parents, tokens, finished_out, history_out, eos, step):
-    groups, beams = scores.shape
-    L = lib()
-    f = L.mmf_beam_select_ws_bytes
-    f.restype = C.c_int64
-    vocab = logits.shape[1]
-    ws = _ws(f(groups, beams, C.c_int64(vocab)), logits.device)
-    d = BeamSelectDesc(_a(logits), logits.stride(0), _a(scores), _a(finished), _a(history), _a(scores_out), _a(parents), _a(tokens), _a(finished_out),
-                       _a(history_out), _a(ws), vocab, eos, 0 if history is None else history.shape[2], step, groups, beams, int(logits.dtype == torch.float32))
-    _check(L.mmf_beam_select(C.byref(d), _stream()), "mmf_beam_select")
-
-
-def paged_reorder(parents, kv_lens, tables, tables_out, copies, page_size):
-    groups, beams = parents.shape
-    d = PagedReorderDesc(_a(parents), _a(kv_lens), _a(tables), _a(tables_out), _a(copies), groups, beams, tables.shape[1], page_size)
-    _check(lib().mmf_paged_reorder(C.byref(d), _stream()), "mmf_paged_reorder")
-
-
-def paged_copy(copies, cache):
-    """cache [..., pages, kv_heads, page_size, head_dim], its leading dimensions one stride apart (or none)."""
-    planes = cache.flatten(0, -5) if cache.dim() > 4 else cache.unsqueeze(0)
-    n, pages, heads, page_size, dim = planes.shape
-    d = PagedCopyDesc(_a(copies), _a(cache), planes.stride(0), planes.stride(1), planes.stride(2), planes.stride(3), copies.shape[0], n, pages, page_size, heads,
-                      dim, int(cache.dtype == torch.float32))
-    _check(lib().mmf_paged_copy(C.byref(d), _stream()), "mmf_paged_copy")
