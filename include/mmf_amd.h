@@ -772,10 +772,10 @@ typedef struct mmf_paged_plan_desc {
     int32_t* tables; int32_t* owned;             /* [groups * beams, blocks]; owned: the page each row took for each of its blocks, -1 none */
     int32_t* free_pages; const int32_t* free_top;
     int32_t* q_start; int32_t* granted; int32_t* kv_out; int64_t* slots; int32_t* positions; int32_t* copies /* [groups * beams, 3] */; int32_t* top_out; int32_t* refused;
-    void* ws;                                    /* mmf_paged_plan_ws_bytes(groups) bytes, 16-byte aligned */
+    void* ws;                                    /* mmf_paged_plan_ws_bytes(groups, beams) bytes, 16-byte aligned */
     int groups, beams, blocks, page_size, rows, shared, free_capacity;
 } mmf_paged_plan_desc;
-int64_t mmf_paged_plan_ws_bytes(int groups);
+int64_t mmf_paged_plan_ws_bytes(int groups, int beams);
 int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream);
 /* k / v row t, head h at t * k_row + h * k_head (elements) -> slot slots[t] of the caches; slots[t] < 0: skipped.  bf16 or fp32 throughout. */
 typedef struct mmf_paged_write_desc {

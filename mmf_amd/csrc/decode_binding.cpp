@@ -104,7 +104,7 @@ Plan plan_pages(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& table
     check_dense(free_pages, "free_pages", at::kInt, {-1});
     check_dense(free_top, "free_top", at::kInt, {1});
     NEED(tables.size(1) > 0 && free_pages.numel() > 0, "tables and free_pages must not be empty");
-    NEED(tables.size(1) * page_size <= (1 << 30) && R <= 0x3fffffff && free_pages.numel() <= 0x7fffffff, "a table row names more than 2**30 tokens");
+    NEED(tables.size(1) * page_size <= (1 << 30) && R <= 0x0fffffff && free_pages.numel() <= 0x7fffffff, "a table row names more than 2**30 tokens");
     Plan p;
     if (!out.empty()) {
         NEED(out.size() == 8, "out is a PagePlan");
@@ -127,7 +127,7 @@ Plan plan_pages(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& table
                      pos = c.take({rows}, at::kInt), copies = c.take({R, 3}, at::kInt), top = c.take({1}, at::kInt), refused = c.take({1}, at::kInt);
         p = {start, granted, kv, slots, pos, copies, top, refused};
     }
-    const Tensor ws = workspace(mmf_paged_plan_ws_bytes((int)G), q_lens);
+    const Tensor ws = workspace(mmf_paged_plan_ws_bytes((int)G, (int)beams), q_lens);
     mmf_paged_plan_desc d = {};
     d.q_lens = PT<int32_t>(q_lens); d.kv_lens = PT<int32_t>(kv_lens); d.tables = PT<int32_t>(tables); d.owned = PT<int32_t>(owned);
     d.free_pages = PT<int32_t>(free_pages); d.free_top = PT<int32_t>(free_top);
@@ -215,11 +215,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
     check_dense(scores, "scores", at::kFloat, {-1, -1});
     const int64_t G = scores.size(0), W = scores.size(1);
     check_beams(W);
-    NEED(G > 0 && G * W <= 0x3fffffff, "select_beams needs a group");
+    NEED(G > 0 && G * W <= 65535, "select_beams needs 1 .. 65535 rows in groups, got ", G * W);
     check_float(logits, "logits");
     NEED(logits.dim() == 2 && logits.size(0) == G * W, "logits must be [", G * W, ", vocab], got ", logits.sizes());
     const int64_t V = logits.size(1);
-    NEED(V > 0 && (logits.stride(1) == 1 || V == 1) && (logits.stride(0) >= V || G * W == 1), "logits must have contiguous rows that do not overlap");
+    NEED(V > 0 && V <= 0x3fffffff && (logits.stride(1) == 1 || V == 1) && (logits.stride(0) >= V || G * W == 1), "logits must have contiguous rows that do not overlap");
     check_dense(finished, "finished", at::kBool, {G, W});
     NEED(eos >= 0 && eos < V, "eos ", eos, " is not in the vocabulary of ", V);
     const Tensor history = history_.has_value() ? *history_ : Tensor();

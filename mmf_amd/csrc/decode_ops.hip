@@ -8,9 +8,7 @@
 
 namespace {
 
-constexpr int PLAN_THREADS = 1024;
-
-// inclusive sum over the workgroup's PLAN_THREADS threads; `total` gets the sum of all
+// inclusive sum over the workgroup; `total` gets the sum of all.  lds: one value per wave
 template <typename T> DEVI T block_scan(T v, int64_t* lds, T& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     T s = v;
@@ -24,8 +22,8 @@ template <typename T> DEVI T block_scan(T v, int64_t* lds, T& total) {
     __syncthreads();
     T before = 0;
     total = 0;
-#pragma unroll
-    for (int w = 0; w < PLAN_THREADS / 64; ++w) {
+#pragma unroll 1
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) {
         const T x = (T)lds[w];
         if (w < wave) before += x;
         total += x;
@@ -34,109 +32,144 @@ template <typename T> DEVI T block_scan(T v, int64_t* lds, T& total) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// the plan of a step.  Whole numbers only; a few bytes per request and 12 per new token: latency is all there is to it.
+// the plan of a step.  Whole numbers only; a few bytes per request and 12 per new token: latency is all there is to it.  One workgroup takes back the pages of
+// finished groups and scans the groups (a thread each: what a group needs, what those before it took); the rows' tokens and blocks are filled in by the
+// same launch where they are few, and by a second one over the whole chip where not.
 // ------------------------------------------------------------------------------------------------
 struct PlanGroup {      // what the scan leaves for the rows of a group
     int base;           // pages taken by the groups before it
     int forks;          // bit w: beam w takes a page for the block it shares so far
     int kv;             // tokens in the cache before this step
-    int granted;        // new tokens, -1: none (released, refused)
+    int granted;        // new tokens; -1 - n: none of the n asked for
 };
 
-DEVI int blocks_of(int tokens, int page_size) { return (int)(((int64_t)tokens + page_size - 1) / page_size); }
+constexpr int PLAN_THREADS = 1024;       // (256 where that is a thread per group)
 
-// pages of released groups, back on the stack in the order of their rows and blocks; returns the new top
-DEVI int plan_release(const mmf_paged_plan_desc& d, int64_t* lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int R = d.groups * d.beams;
-    int top = d.free_top[0];
-    top = min(max(top, 0), d.free_capacity);
-    if (threadIdx.x == 0 && top != d.free_top[0]) flag_page_error();
-    for (int r0 = 0; r0 < R; r0 += PLAN_THREADS / 64) {          // one wave per row: count, place, push
-        const int r = r0 + wave;
-        int n = 0, blocks = 0;
-        if (r < R && d.q_lens[r / d.beams] < 0) {
-            blocks = min(blocks_of(max(d.kv_lens[r / d.beams], 0), d.page_size), d.blocks);
-            for (int j0 = 0; j0 < blocks; j0 += 64) n += __popcll(__ballot(j0 + lane < blocks && d.owned[(size_t)r * d.blocks + j0 + lane] >= 0));
-        }
-        __syncthreads();
-        if (lane == 0) lds[wave] = n;
-        __syncthreads();
-        int at = top, total = 0;
+DEVI int blocks_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
+
+// Pages of released groups, back on the stack in the order of their rows and blocks; returns the new top.  A wave counts a row's pages, the counts are scanned,
+// a wave pushes them; `counts` holds one int per row.
+DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, int* counts, int64_t* lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6, R = d.groups * d.beams;
+#pragma unroll 1
+    for (int r = wave; r < R; r += waves) {
+        int n = 0;
+        const int g = r / d.beams;
+        if (d.q_lens[g] < 0) {
+            const int blocks = min(blocks_of(max(d.kv_lens[g], 0), shift), d.blocks);
+            for (int j = lane; j < blocks; j += 64) n += d.owned[(size_t)r * d.blocks + j] >= 0;
 #pragma unroll
-        for (int w = 0; w < PLAN_THREADS / 64; ++w) {
-            const int x = (int)lds[w];
-            if (w < wave) at += x;
-            total += x;
+            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
         }
-        for (int j0 = 0; j0 < blocks && n > 0; j0 += 64) {
+        if (lane == 0) counts[r] = n;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int r0 = 0; r0 < R; r0 += blockDim.x) {                  // counts[r] becomes the row's place on the stack
+        const int r = r0 + tid, n = r < R ? counts[r] : 0;
+        int total;
+        const int upto = block_scan(n, lds, total);
+        if (r < R) counts[r] = n ? top + upto - n : -1;
+        top = min(top + total, d.free_capacity);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int r = wave; r < R; r += waves) {
+        int at = counts[r];
+        if (at < 0) continue;
+        const int blocks = min(blocks_of(max(d.kv_lens[r / d.beams], 0), shift), d.blocks);
+        for (int j0 = 0; j0 < blocks; j0 += 64) {
             const int p = j0 + lane < blocks ? d.owned[(size_t)r * d.blocks + j0 + lane] : -1;
             const uint64_t m = __ballot(p >= 0);
             const int to = at + __popcll(m & ((1ull << lane) - 1));
             if (p >= 0) {
                 if (to < d.free_capacity) d.free_pages[to] = p;
-                else flag_page_error();                          // more pages came back than the pool has: a page was given back twice
+                else flag_page_error();                          // more pages came back than the pool has: one was given back twice
             }
             at += __popcll(m);
         }
-        top = min(top + total, d.free_capacity);
     }
+    __syncthreads();
     return top;
 }
 
 // the tokens and blocks of one row, by `nthr` threads
-DEVI void plan_row(const mmf_paged_plan_desc& d, const PlanGroup& g, int r, int start, int top, int tid, int nthr) {
-    const int w = r % d.beams, ps = d.page_size;
-    const bool first = w == 0;
+DEVI void plan_row(const mmf_paged_plan_desc& d, int shift, const PlanGroup& g, int r, int w, int start, int top, int tid, int nthr) {
+    const bool gets = !d.shared || w == 0;                        // has tokens and pages of its own
     if (g.granted > 0) {
-        const int have = blocks_of(g.kv, ps), want = blocks_of(g.kv + g.granted, ps);
+        const int have = blocks_of(g.kv, shift), want = blocks_of(g.kv + g.granted, shift), below = (1 << shift) - 1;
         const bool fork = (g.forks >> w) & 1;
-        const int lo = fork ? g.kv / ps : have;
+        const int lo = fork ? g.kv >> shift : have;
         int rank = g.base;                                        // the row's first page, counted from the top of the stack
         if (!d.shared) rank += w * (want - have) + __popc(g.forks & ((1u << w) - 1u));
+        const int* from = d.free_pages + (top - 1 - rank + lo);   // from[-j]: the page of block j >= lo
         int* table = d.tables + (size_t)r * d.blocks;
         int* owned = d.owned + (size_t)r * d.blocks;
-        for (int j = lo + tid; j < want; j += nthr) {
-            const int page = d.free_pages[top - 1 - (rank + j - lo)];
-            if (fork && j == lo) { d.copies[3 * r] = table[j]; d.copies[3 * r + 1] = page; d.copies[3 * r + 2] = g.kv % ps; }
-            table[j] = page;
-            owned[j] = (!d.shared || first) ? page : -1;          // a shared block belongs to the group's first row
-        }
-        if (!d.shared || first) {
+        const int part = have > 0 ? table[have - 1] : -1;         // the block that is not full yet, unless the row gets a page for it
+        if (gets)
             for (int i = tid; i < g.granted; i += nthr) {
-                const int pos = g.kv + i, j = pos / ps;
-                const int page = j >= lo ? d.free_pages[top - 1 - (rank + j - lo)] : table[j];
-                d.slots[start + i] = page < 0 ? -1 : (int64_t)page * ps + (pos - j * ps);
+                const int pos = g.kv + i, j = pos >> shift;
+                const int page = j >= lo ? from[-j] : part;
+                d.slots[start + i] = page < 0 ? -1 : ((int64_t)page << shift) + (pos & below);
                 d.positions[start + i] = pos;
             }
+        for (int j = lo + tid; j < want; j += nthr) {
+            const int page = from[-j];
+            if (fork && j == lo) {
+                int* c = d.copies + 3 * (size_t)r;
+                c[0] = part; c[1] = page; c[2] = g.kv & below;
+            }
+            table[j] = page;
+            owned[j] = gets ? page : -1;                          // a shared block belongs to the group's first row
         }
-    } else if (!d.shared || first) {                              // the tokens of a request that has to wait
+    } else if (gets) {                                            // the tokens of a request that has to wait
         const int n = min(-1 - g.granted, d.rows - start);
         for (int i = tid; i < n; i += nthr) { d.slots[start + i] = -1; d.positions[start + i] = -1; }
     }
 }
 
-__global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc d) {
+// rows_too: a row by one thread, or by eight where some have more than four tokens; else the second launch takes a wave per row
+__global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc d, int shift, int rows_too) {
     __shared__ int64_t lds[PLAN_THREADS / 64];
-    const int tid = threadIdx.x, W = d.beams, ps = d.page_size, per = d.shared ? 1 : W;
+    __shared__ int taken, refused, flags;                         // flags: 1 a group is released, 2 a row has many tokens
+    const int tid = threadIdx.x, threads = blockDim.x, W = d.beams, per = d.shared ? 1 : W;
     PlanGroup* ws = reinterpret_cast<PlanGroup*>(d.ws);
-    const int top = plan_release(d, lds);
-    int carry_need = 0, carry_refused = 0, carry_taken = 0, total;
-    int64_t carry_rows = 0, total_rows;
-    for (int g0 = 0; g0 < d.groups; g0 += PLAN_THREADS) {
+    int* tail = reinterpret_cast<int*>(ws + d.groups);             // [0]: the top the pages are taken from, [4 ..]: plan_release's counts
+    if (tid == 0) { taken = 0; refused = 0; flags = 0; }
+    for (int i = tid; i < 3 * d.groups * W; i += threads) d.copies[i] = -1;
+    const int told = d.free_top[0];
+    int top = min(max(told, 0), d.free_capacity);
+    if (tid == 0 && top != told) flag_page_error();
+    __syncthreads();
+    int most = 0, least = 0;
+    for (int g = tid; g < d.groups; g += threads) {
+        const int q = d.q_lens[g];
+        most = max(most, q);
+        least = min(least, q);
+    }
+    const int f = (least < 0) | (most > 4) << 1;
+    if (f) atomicOr(&flags, f);
+    __syncthreads();
+    if (flags & 1) top = plan_release(d, shift, top, tail + 4, lds);
+    const int per_row = flags & 2 ? 8 : 1;
+    int carry_need = 0, total;
+    int64_t carry_rows = 0, total64;
+#pragma unroll 1
+    for (int g0 = 0; g0 < d.groups; g0 += threads) {
         const int g = g0 + tid;
         const bool in = g < d.groups;
         const int q = in ? d.q_lens[g] : 0, kv = in ? max(d.kv_lens[g], 0) : 0, n = max(q, 0);
-        const int64_t rows = (int64_t)per * n, start64 = carry_rows + block_scan(rows, lds, total_rows) - rows;
-        carry_rows += total_rows;
-        const bool fits = (int64_t)kv + n <= (int64_t)d.blocks * ps && start64 + rows <= d.rows;
+        const int64_t rows = (int64_t)per * n, start = carry_rows + block_scan(rows, lds, total64) - rows;
+        carry_rows += total64;
+        const bool fits = (int64_t)kv + n <= (int64_t)d.blocks << shift && start + rows <= d.rows;
         int need = 0, forks = 0;
-        if (in && n > 0 && fits) {
-            const int fresh = blocks_of(kv + n, ps) - blocks_of(kv, ps);
-            if (!d.shared && kv % ps != 0)
-                for (int w = 1; w < W; ++w)
-                    if (d.owned[((size_t)g * W + w) * d.blocks + kv / ps] < 0) forks |= 1 << w;
-            need = per * fresh + __popc(forks);
+        if (n > 0 && fits) {
+            if (!d.shared && (kv & ((1 << shift) - 1))) {
+                const int* owned = d.owned + (size_t)g * W * d.blocks + (kv >> shift);
+#pragma unroll 4
+                for (int w = 1; w < W; ++w) forks |= (owned[(size_t)w * d.blocks] < 0) << w;
+            }
+            need = per * (blocks_of(kv + n, shift) - blocks_of(kv, shift)) + __popc(forks);
         }
         const int upto = carry_need + block_scan(need, lds, total);
         carry_need += total;
@@ -145,25 +178,31 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc 
             d.granted[g] = served ? n : 0;
             d.kv_out[g] = q < 0 ? 0 : kv + (served ? n : 0);
             ws[g] = PlanGroup{upto - need, served ? forks : 0, kv, served ? n : -1 - n};
-            for (int w = 0; w < per; ++w) d.q_start[(size_t)g * per + w] = (int)min(start64 + (int64_t)w * n, (int64_t)d.rows);
+            for (int w = 0; w < per; ++w) d.q_start[(size_t)g * per + w] = (int)min(start + (int64_t)w * n, (int64_t)d.rows);
+            if (served && need) atomicMax(&taken, upto);          // (all that is asked for before a group that gets pages is served too)
+            if (q >= 0 && !served) atomicAdd(&refused, 1);
         }
-        block_scan(served ? need : 0, lds, total);
-        carry_taken += total;
-        block_scan((int)(in && q >= 0 && !served), lds, total);
-        carry_refused += total;
     }
-    if (tid == 0) {
-        d.top_out[0] = top - carry_taken;
-        d.refused[0] = carry_refused;
-    }
-    for (int i = tid; i < 3 * d.groups * W; i += PLAN_THREADS) d.copies[i] = -1;
-    for (int64_t i = carry_rows + tid; i < d.rows; i += PLAN_THREADS) { d.slots[i] = -1; d.positions[i] = -1; }
+    for (int64_t i = carry_rows + tid; i < d.rows; i += threads) { d.slots[i] = -1; d.positions[i] = -1; }
     __syncthreads();
-    const int lane = tid & 63;
-    for (int r = tid >> 6; r < d.groups * W; r += PLAN_THREADS / 64) {
-        const int g = r / W;
-        plan_row(d, ws[g], r, d.shared ? d.q_start[g] : d.q_start[r], top, lane, 64);
+    if (tid == 0) {
+        d.top_out[0] = top - taken;
+        d.refused[0] = refused;
+        tail[0] = top;
     }
+    if (!rows_too) return;
+#pragma unroll 1
+    for (int r = tid / per_row; r < d.groups * W; r += threads / per_row) {
+        const int g = r / W;
+        plan_row(d, shift, ws[g], r, r - g * W, d.shared ? d.q_start[g] : d.q_start[r], top, tid % per_row, per_row);
+    }
+}
+__global__ __launch_bounds__(256) void plan_rows_kernel(mmf_paged_plan_desc d, int shift) {
+    const PlanGroup* ws = reinterpret_cast<const PlanGroup*>(d.ws);
+    const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= d.groups * d.beams) return;
+    const int g = r / d.beams;
+    plan_row(d, shift, ws[g], r, r - g * d.beams, d.shared ? d.q_start[g] : d.q_start[r], reinterpret_cast<const int*>(ws + d.groups)[0], threadIdx.x & 63, 64);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -195,92 +234,325 @@ __global__ __launch_bounds__(256) void paged_write_kernel(mmf_paged_write_desc d
 // the best continuations of a group.  Candidate (w, v) of an unfinished beam: score[w] + logit[w][v] - lse[w]; of a finished one: the
 // end token at score[w].  The W largest, the lowest flat index w * V + v first among equals.  Values of different beams meet in 64 bits:
 // in 32 the sum would round candidates together that are apart.
+//
+// Within a row the order is the logits' own, so a first kernel takes every row in segments, a workgroup each, and leaves the segment's maximum, its sum of exponentials
+// and its W largest; a second one merges the segments and beams of a group.  Both pick W out of N in the same way: the W-th largest of a wave's 64 lane
+// maxima is a bar that at least W values reach, and few more do; those are ranked by counting.  The second look at a segment comes from the caches.
+// Loops stay rolled: a launch that runs its code once waits for the instructions more than for anything else.
 // ------------------------------------------------------------------------------------------------
 constexpr double NEG_INF = -__builtin_huge_val();
+constexpr int SEG_MAX = 8192, LIST = 1024;
 
-struct Cand { double v; int64_t i; };
+struct Picked { float v; int i; };                                // i: index in the row, -1: none
+struct Segment { double sum; float top; int pad; };               // sum of exp(x - top)
 DEVI bool better(double av, int64_t ai, double bv, int64_t bi) { return av > bv || (av == bv && ai < bi); }
 
-template <typename T> DEVI float logit(const T* x, int64_t v) {
-    const float f = (float)x[v];
-    return f == f ? f : -INFINITY;
+// the W-th largest of a wave's 64 values
+DEVI float wave_bar(float mine, int W, int lane) {
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) {
+        const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), j));
+        rank += x > mine || (x == mine && j < lane);
+    }
+    return __shfl(mine, __ffsll((unsigned long long)__ballot(rank == W - 1)) - 1, 64);
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void beam_select_kernel(mmf_beam_select_desc d) {
-    __shared__ double red_v[4], lse[MMF_BEAMS_MAX], score[MMF_BEAMS_MAX];
-    __shared__ int64_t red_i[4], token[MMF_BEAMS_MAX];
-    __shared__ int parent[MMF_BEAMS_MAX], done[MMF_BEAMS_MAX];
-    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W = d.beams;
-    const int64_t V = d.vocab;
-    if (tid < W) {                                                // (scores and finished may be updated in place)
-        score[tid] = (double)d.scores[g * W + tid];
-        done[tid] = d.finished[g * W + tid] != 0;
-    }
-    for (int w = 0; w < W; ++w) {
-        const T* x = (const T*)d.logits + ((size_t)g * W + w) * d.ld;
-        float m = -INFINITY;
-        for (int64_t v = tid; v < V; v += 256) m = fmaxf(m, logit(x, v));
-        m = wave_max(m);
-        __syncthreads();
-        if (lane == 0) red_v[wave] = m;
-        __syncthreads();
-        m = (float)fmax(fmax(red_v[0], red_v[1]), fmax(red_v[2], red_v[3]));
-        double s = 0.0;
-        if (m > -INFINITY)
-            for (int64_t v = tid; v < V; v += 256) s += (double)expf(logit(x, v) - m);
+// exp(x) for x <= 0, the rounding of x log2 e carried along: relative 2^-23 at any x
+DEVI float exp_down(float x) {
+    x = fmaxf(x, -200.f);                                         // (a masked value: its power is 0 all the same)
+    const float a = x * 1.44269504088896340736f, r = fmaf(x, 1.9259629911266174e-8f, fmaf(x, 1.44269504088896340736f, -a));
+    return __builtin_amdgcn_exp2f(a) * fmaf(r, 0.693147180559945309f, 1.f);
+}
+// log(x) of a normal x > 0 in 64 bits: x = m 2^e with m in [sqrt 1/2, sqrt 2), log m = 2 atanh(s), s = (m - 1) / (m + 1), |s| < 0.172: the series ends below 1e-13
+DEVI double log_of(double x) {
+    int e = __builtin_amdgcn_frexp_exp(x);
+    double m = __builtin_amdgcn_frexp_mant(x);
+    if (m < 0.70710678118654752) { m *= 2.0; e -= 1; }
+    const double s = (m - 1.0) / (m + 1.0), q = s * s;
+    double p = 1.0 / 15.0;
+#pragma unroll 1
+    for (int k = 13; k >= 1; k -= 2) p = p * q + 1.0 / k;
+    return 2.0 * s * p + e * 0.69314718055994530942;
+}
+
+// 16 bytes of a row as floats, NaN as -inf; WIDE: rows start on 4 bytes, else on an element
+template <typename T, bool WIDE> struct Reader {
+    static constexpr int VEC = 16 / (int)sizeof(T);
+    typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(4)));
+    DEVI static void load(const T* x, int at, int n, float (&v)[VEC]) {
+        T raw[VEC];
+        if (WIDE && at + VEC <= n) {
+            const u32x4a w = *reinterpret_cast<const u32x4a*>(x + at);
+            __builtin_memcpy(raw, &w, 16);
+        } else {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-        __syncthreads();
-        if (lane == 0) red_v[wave] = s;
-        __syncthreads();
-        if (tid == 0) lse[w] = (double)m + log(red_v[0] + red_v[1] + red_v[2] + red_v[3]);
+            for (int e = 0; e < VEC; ++e) raw[e] = at + e < n ? x[at + e] : (T)-INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float f = (float)raw[e];
+            v[e] = f == f ? f : -INFINITY;
+        }
     }
+};
+
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void beam_rows_kernel(mmf_beam_select_desc d, int segments, int length) {
+    typedef Reader<T, WIDE> R;
+    constexpr int VEC = R::VEC;
+    __shared__ float cand_v[LIST], tops[4], bars[4];
+    __shared__ int cand_i[LIST], count;
+    __shared__ double sums[4];
+    const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W = d.beams;
+    const float score = d.scores[row];
+    if (d.finished[row] || !(score > -INFINITY)) return;          // (the second kernel does not look at these rows either)
+    const int64_t first = (int64_t)seg * length;
+    const int n = (int)min((int64_t)length, d.vocab - first);
+    const T* x = (const T*)d.logits + (int64_t)row * d.ld + first;
+    if (tid == 0) count = 0;
+    float mine = -INFINITY;
+#pragma unroll 4
+    for (int at = tid * VEC; at < n; at += 256 * VEC) {
+        float v[VEC];
+        R::load(x, at, n, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) mine = fmaxf(mine, v[e]);
+    }
+    const float b = wave_bar(mine, W, lane), t = wave_max(mine);
+    if (lane == 0) { tops[wave] = t; bars[wave] = b; }
     __syncthreads();
-    double last_v = -NEG_INF;
-    int64_t last_i = -1;
-    for (int k = 0; k < W; ++k) {                                 // the best candidate behind the last one chosen
-        double bv = NEG_INF;
-        int64_t bi = INT64_MAX;
-        for (int w = 0; w < W; ++w) {
-            const T* x = (const T*)d.logits + ((size_t)g * W + w) * d.ld;
-            for (int64_t v = tid; v < V; v += 256) {
-                double c = done[w] ? (v == d.eos ? score[w] : NEG_INF) : score[w] + ((double)logit(x, v) - lse[w]);
-                if (!(c == c)) c = NEG_INF;
-                const int64_t i = w * V + v;
-                if (better(last_v, last_i, c, i) && better(c, i, bv, bi)) { bv = c; bi = i; }
+    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float bar = fmaxf(fmaxf(bars[0], bars[1]), fmaxf(bars[2], bars[3]));
+    const float base = top > -INFINITY && top < INFINITY ? top : 0.f;
+    double s = 0.0;
+#pragma unroll 1
+    for (int at = tid * VEC; at < n; at += 256 * VEC) {
+        float v[VEC];
+        R::load(x, at, n, v);
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+            s += (double)((exp_down(v[e] - base) + exp_down(v[e + 1] - base)) + (exp_down(v[e + 2] - base) + exp_down(v[e + 3] - base)));
+            any |= fmaxf(fmaxf(v[e], v[e + 1]), fmaxf(v[e + 2], v[e + 3])) >= bar;
+        }
+        if (any) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (v[e] >= bar && v[e] > -INFINITY) {
+                    const int to = atomicAdd(&count, 1);
+                    if (to < LIST) { cand_v[to] = v[e]; cand_i[to] = at + e; }
+                }
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) sums[wave] = s;
+    __syncthreads();
+    Picked* out = (Picked*)d.ws + ((int64_t)row * segments + seg) * W;
+    Segment* seg_out = (Segment*)((Picked*)d.ws + (((int64_t)d.groups * W * segments * W + 1) & ~1ll)) + (int64_t)row * segments + seg;
+    if (tid == 0) *seg_out = Segment{sums[0] + sums[1] + sums[2] + sums[3], top, 0};
+    const int found = count;
+    if (found <= LIST) {
+        for (int i = tid; i < found; i += 256) {
+            const float a = cand_v[i];
+            const int ai = cand_i[i];
+            int rank = 0;
+            for (int j = 0; j < found; ++j) {
+                const float bv = cand_v[j];
+                rank += bv > a || (bv == a && cand_i[j] < ai);
             }
+            if (rank < W) out[rank] = Picked{a, (int)first + ai};
+        }
+        if (tid >= found && tid < W) out[tid] = Picked{-INFINITY, -1};
+        return;
+    }
+    float last = INFINITY;                                        // a plateau of equal values wider than the list: one round per value picked
+    int last_i = -1;
+#pragma unroll 1
+    for (int k = 0; k < W; ++k) {
+        float bv = -INFINITY;
+        int bi = 0x7fffffff;
+#pragma unroll 1
+        for (int i = tid; i < n; i += 256) {
+            const float f = (float)x[i], y = f == f ? f : -INFINITY;
+            if (y > -INFINITY && (y < last || (y == last && i > last_i)) && (y > bv || (y == bv && i < bi))) { bv = y; bi = i; }
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
-            const double ov = __shfl_xor(bv, o, 64);
-            const int64_t oi = __shfl_xor((long long)bi, o, 64);
-            if (better(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+            const float ov = __shfl_xor(bv, o, 64);
+            const int oi = __shfl_xor(bi, o, 64);
+            if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
         }
         __syncthreads();
-        if (lane == 0) { red_v[wave] = bv; red_i[wave] = bi; }
+        if (lane == 0) { cand_v[wave] = bv; cand_i[wave] = bi; }
         __syncthreads();
         for (int u = 0; u < 4; ++u)
-            if (u == 0 || better(red_v[u], red_i[u], bv, bi)) { bv = red_v[u]; bi = red_i[u]; }
-        last_v = bv;
+            if (cand_v[u] > bv || (cand_v[u] == bv && cand_i[u] < bi)) { bv = cand_v[u]; bi = cand_i[u]; }
+        last = bv;
         last_i = bi;
-        if (tid == 0) {
-            const int p = (int)(bi / V);
-            parent[k] = p;
-            token[k] = bi - (int64_t)p * V;
-            d.scores_out[g * W + k] = (float)bv;
-            d.parents[g * W + k] = p;
-            d.tokens[g * W + k] = token[k];
+        if (tid == 0) out[k] = bi == 0x7fffffff ? Picked{-INFINITY, -1} : Picked{bv, (int)first + bi};
+    }
+}
+
+__global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d, int segments) {
+    __shared__ double cand_v[LIST], score[MMF_BEAMS_MAX], lse[MMF_BEAMS_MAX], best_v[MMF_BEAMS_MAX], red_v[4];
+    __shared__ int64_t cand_i[LIST], best_i[MMF_BEAMS_MAX], red_i[4];
+    __shared__ int done[MMF_BEAMS_MAX], parent[MMF_BEAMS_MAX], count;
+    __shared__ float bars[4];
+    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W = d.beams;
+    const int64_t V = d.vocab;
+    const Picked* picked = (const Picked*)d.ws + (int64_t)g * W * segments * W;
+    const Segment* segs = (const Segment*)((const Picked*)d.ws + (((int64_t)d.groups * W * segments * W + 1) & ~1ll)) + (int64_t)g * W * segments;
+    if (tid < W) {                                                // (scores and finished may be updated in place)
+        const float s = d.scores[g * W + tid];
+        score[tid] = s == s ? (double)s : NEG_INF;
+        done[tid] = d.finished[g * W + tid] != 0;
+        best_v[tid] = NEG_INF;
+        best_i[tid] = -1;
+    }
+    if (tid == 0) count = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int w = wave; w < W; w += 4) {                           // lse: NaN marks a row without candidates
+        if (done[w] || !(score[w] > NEG_INF)) {
+            if (lane == 0) lse[w] = __builtin_nan("");
+            continue;
+        }
+        float m = -INFINITY;
+        for (int s = lane; s < segments; s += 64) m = fmaxf(m, segs[w * segments + s].top);
+        m = wave_max(m);
+        double sum = 0.0;
+        for (int s = lane; s < segments; s += 64) {
+            const Segment x = segs[w * segments + s];
+            if (x.top > -INFINITY) sum += x.sum * (double)exp_down(x.top - m);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        const double z = log_of(sum);
+        if (lane == 0) lse[w] = m > -INFINITY && m < INFINITY ? (double)m + z : __builtin_nan("");
+    }
+    __syncthreads();
+    // candidate k of beam w's lists; a finished beam's only one stands first in its lists
+    const int per = segments * W;
+    auto cand = [&](int w, int k, int64_t& i) {
+        double v = NEG_INF;
+        i = w * V;
+        if (done[w]) {
+            if (k == 0) { v = score[w]; i += d.eos; }
+        } else if (lse[w] == lse[w]) {
+            const Picked p = picked[w * per + k];
+            if (p.i >= 0) { v = score[w] + ((double)p.v - lse[w]); i += p.i; }
+        }
+        return v;
+    };
+    float mine = -INFINITY;                                       // (rounding to 32 bits keeps the order)
+#pragma unroll 1
+    for (int k = tid; k < W * per; k += 256) {
+        int64_t i;
+        mine = fmaxf(mine, (float)cand(k / per, k % per, i));
+    }
+    const float b = wave_bar(mine, W, lane);
+    if (lane == 0) bars[wave] = b;
+    __syncthreads();
+    const float bar = fmaxf(fmaxf(bars[0], bars[1]), fmaxf(bars[2], bars[3]));
+    if (mine >= bar)
+#pragma unroll 1
+        for (int k = tid; k < W * per; k += 256) {
+            int64_t i;
+            const double v = cand(k / per, k % per, i);
+            if (v > NEG_INF && (float)v >= bar) {
+                const int to = atomicAdd(&count, 1);
+                if (to < LIST) { cand_v[to] = v; cand_i[to] = i; }
+            }
+        }
+    __syncthreads();
+    const int found = count;
+    if (found <= LIST) {
+        for (int a = tid; a < found; a += 256) {
+            const double v = cand_v[a];
+            const int64_t i = cand_i[a];
+            int rank = 0;
+            for (int b = 0; b < found; ++b) rank += better(cand_v[b], cand_i[b], v, i);
+            if (rank < W) { best_v[rank] = v; best_i[rank] = i; }
+        }
+    } else {
+        double last = -NEG_INF;
+        int64_t last_i = -1;
+#pragma unroll 1
+        for (int r = 0; r < W; ++r) {
+            double bv = NEG_INF;
+            int64_t bi = INT64_MAX;
+#pragma unroll 1
+            for (int k = tid; k < W * per; k += 256) {
+                int64_t i;
+                const double v = cand(k / per, k % per, i);
+                if (v > NEG_INF && better(last, last_i, v, i) && better(v, i, bv, bi)) { bv = v; bi = i; }
+            }
+#pragma unroll 1
+            for (int o = 32; o > 0; o >>= 1) {
+                const double ov = __shfl_xor(bv, o, 64);
+                const int64_t oi = __shfl_xor((long long)bi, o, 64);
+                if (better(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+            }
+            __syncthreads();
+            if (lane == 0) { red_v[wave] = bv; red_i[wave] = bi; }
+            __syncthreads();
+            for (int u = 0; u < 4; ++u)
+                if (better(red_v[u], red_i[u], bv, bi)) { bv = red_v[u]; bi = red_i[u]; }
+            last = bv;
+            last_i = bi;
+            if (tid == 0 && bi != INT64_MAX) { best_v[r] = bv; best_i[r] = bi; }
         }
     }
     __syncthreads();
-    if (tid < W) d.finished_out[g * W + tid] = done[parent[tid]] || token[tid] == d.eos;
-    if (d.history)
-        for (int64_t t = tid; t < d.length; t += 256) {           // a column at a time: in place as well
-            int64_t h[MMF_BEAMS_MAX];
-            for (int w = 0; w < W; ++w) h[w] = t == d.step ? token[w] : d.history[((size_t)g * W + parent[w]) * d.length + t];
-            for (int w = 0; w < W; ++w) d.history_out[((size_t)g * W + w) * d.length + t] = h[w];
+    if (tid == 0 && best_i[W - 1] < 0) {                          // fewer live candidates than beams: the others are equal, the lowest indices go first
+        int have = 0;
+        while (best_i[have] >= 0) ++have;
+        int64_t i = 0;
+        for (int r = have; r < W; ++i) {
+            bool used = false;
+            for (int b = 0; b < have; ++b) used |= best_i[b] == i;
+            if (!used) best_i[r++] = i;
         }
+    }
+    __syncthreads();
+    if (tid < W) {
+        const int64_t i = best_i[tid];
+        const int p = (int)(i / V);
+        const int64_t token = i - p * V;
+        parent[tid] = p;
+        best_i[tid] = token;
+        d.scores_out[g * W + tid] = (float)best_v[tid];
+        d.parents[g * W + tid] = p;
+        d.tokens[g * W + tid] = token;
+        d.finished_out[g * W + tid] = done[p] || token == d.eos;
+    }
+    __syncthreads();
+    if (!d.history) return;
+    const int64_t at = (int64_t)g * W * d.length;
+    constexpr int COLS = 32;                                      // through LDS, 32 columns at a time: in place as well
+    for (int64_t t0 = 0; t0 < d.length; t0 += COLS) {
+        for (int k = tid; k < W * COLS; k += 256) {
+            const int w = k / COLS;
+            const int64_t t = t0 + k % COLS;
+            if (t < d.length) cand_i[k] = t == d.step ? best_i[w] : d.history[at + parent[w] * d.length + t];
+        }
+        __syncthreads();
+        for (int k = tid; k < W * COLS; k += 256)
+            if (t0 + k % COLS < d.length) d.history_out[at + k / COLS * d.length + t0 + k % COLS] = cand_i[k];
+        __syncthreads();
+    }
+}
+
+// Segments of a row: up to 8192 values, and shorter ones where few rows would leave compute units idle (four workgroups for each), down to 1024 values
+int beam_segments(int rows, int64_t vocab, int* length) {
+    const int64_t least = (vocab + SEG_MAX - 1) / SEG_MAX, fill = (1024 + rows - 1) / rows, most = vocab / 1024;
+    int64_t n = fill < most ? fill : most;
+    if (n < least) n = least;
+    const int64_t len = ((vocab + n - 1) / n + 7) / 8 * 8;
+    *length = (int)len;
+    return (int)((vocab + len - 1) / len);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -356,17 +628,27 @@ int mmf_decode_take_error(void) {
     return v;
 }
 
-int64_t mmf_paged_plan_ws_bytes(int groups) { return (int64_t)(groups > 0 ? groups : 0) * (int64_t)sizeof(PlanGroup) + 16; }
+int64_t mmf_paged_plan_ws_bytes(int groups, int beams) {
+    return groups > 0 && beams > 0 ? (int64_t)groups * (int64_t)sizeof(PlanGroup) + 16 + 4 * (int64_t)groups * beams : 0;
+}
 
 int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream) {
     MMF_CHECK_ARG(d && d->q_lens && d->kv_lens && d->tables && d->owned && d->free_pages && d->free_top, "paged_plan: null operand");
     MMF_CHECK_ARG(d->q_start && d->granted && d->kv_out && d->slots && d->positions && d->copies && d->top_out && d->refused && d->ws, "paged_plan: null output");
     MMF_CHECK_ARG(d->groups > 0 && d->blocks > 0 && d->rows > 0 && d->free_capacity > 0, "paged_plan: bad shape");
-    MMF_CHECK_ARG(d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->groups <= 0x3fffffff / d->beams, "paged_plan: 1 .. 32 beams");
+    MMF_CHECK_ARG(d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->groups <= 0x0fffffff / d->beams, "paged_plan: 1 .. 32 beams");
     MMF_CHECK_ARG(d->page_size >= 1 && d->page_size <= MMF_PAGE_MAX && (d->page_size & (d->page_size - 1)) == 0, "paged_plan: page_size is a power of two up to 1024");
-    MMF_CHECK_ARG((int64_t)d->blocks * d->page_size <= 0x3fffffff && d->rows <= 0x3fffffff, "paged_plan: more than 2^30 tokens");
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (hipStream_t)stream, *d);
+    MMF_CHECK_ARG((int64_t)d->blocks * d->page_size <= 0x40000000 && d->rows <= 0x40000000, "paged_plan: more than 2^30 tokens");
+    // one workgroup walks up to a thousand tokens, or a few for each of as many rows as it has threads; more is work for the whole chip and a second launch
+    const int64_t rows = (int64_t)d->groups * d->beams;
+    const bool one = d->rows <= 1024 || (d->rows <= 4 * rows && rows <= 4 * PLAN_THREADS);
+    const int shift = __builtin_ctz(d->page_size);
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(rows <= 256 ? 256 : PLAN_THREADS), 0, (hipStream_t)stream, *d, shift, (int)one);
     MMF_CHECK_LAUNCH();
+    if (!one) {
+        hipLaunchKernelGGL(plan_rows_kernel, dim3((d->groups * d->beams + 3) / 4), dim3(256), 0, (hipStream_t)stream, *d, shift);
+        MMF_CHECK_LAUNCH();
+    }
     return 0;
 }
 
@@ -389,15 +671,28 @@ int mmf_paged_write(const mmf_paged_write_desc* d, void* stream) {
     return 0;
 }
 
-int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab) { (void)groups; (void)beams; (void)vocab; return 0; }
+int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab) {
+    if (groups < 1 || beams < 1 || vocab < 1) return 0;
+    int length;
+    const int64_t rows = (int64_t)groups * beams, n = beam_segments((int)rows, vocab, &length);
+    return ((rows * n * beams + 1) & ~1ll) * (int64_t)sizeof(Picked) + rows * n * (int64_t)sizeof(Segment);
+}
 
 int mmf_beam_select(const mmf_beam_select_desc* d, void* stream) {
-    MMF_CHECK_ARG(d && d->logits && d->scores && d->finished && d->scores_out && d->parents && d->tokens && d->finished_out, "beam_select: null operand");
+    MMF_CHECK_ARG(d && d->logits && d->scores && d->finished && d->scores_out && d->parents && d->tokens && d->finished_out && d->ws, "beam_select: null operand");
     MMF_CHECK_ARG(d->groups > 0 && d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->vocab > 0 && d->ld >= d->vocab, "beam_select: bad shape");
+    MMF_CHECK_ARG(d->vocab <= 0x3fffffff && (int64_t)d->groups * d->beams <= 65535, "beam_select: 2^30 tokens and 65535 rows at most");
     MMF_CHECK_ARG(d->eos >= 0 && d->eos < d->vocab, "beam_select: the end token is not in the vocabulary");
     MMF_CHECK_ARG(!d->history || (d->history_out && d->length > 0 && d->step >= 0 && d->step < d->length), "beam_select: step is not a column of the history");
-    if (d->is_f32) hipLaunchKernelGGL(beam_select_kernel<float>, dim3(d->groups), dim3(256), 0, (hipStream_t)stream, *d);
-    else hipLaunchKernelGGL(beam_select_kernel<bf16>, dim3(d->groups), dim3(256), 0, (hipStream_t)stream, *d);
+    int length;
+    const int segments = beam_segments(d->groups * d->beams, d->vocab, &length);
+    const dim3 grid(segments, d->groups * d->beams);
+    const bool wide = ((uintptr_t)d->logits & 3) == 0 && (d->ld & 1) == 0;
+    if (d->is_f32) hipLaunchKernelGGL((beam_rows_kernel<float, true>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
+    else if (wide) hipLaunchKernelGGL((beam_rows_kernel<bf16, true>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
+    else hipLaunchKernelGGL((beam_rows_kernel<bf16, false>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
+    MMF_CHECK_LAUNCH();
+    hipLaunchKernelGGL(beam_merge_kernel, dim3(d->groups), dim3(256), 0, (hipStream_t)stream, *d, segments);
     MMF_CHECK_LAUNCH();
     return 0;
 }

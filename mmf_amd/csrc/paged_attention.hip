@@ -23,6 +23,7 @@ typedef __attribute__((address_space(3))) void* lds_vp;
 typedef const __attribute__((address_space(1))) void* glb_vp;
 static __device__ uint4 g_zero16;
 
+constexpr int STEP_ROWS = 32, CHUNK_ROWS = 128;
 constexpr int UNITS_MAX = 1024;        // requests (chunks) or groups of beams (steps) per launch
 constexpr int PREFIX_MAX = 3 * (UNITS_MAX + 1) * 4;
 
@@ -31,8 +32,9 @@ struct Args {
     int page_shift, group;             // group: query heads per key head
     int units, nb, per_group;          // nb: beams a unit takes together (steps), per_group: units per group of beams
     int target, run_min;               // workgroups to aim at when keys are split; shortest run
+    int split, tiles;                  // whether keys may be split at all; row tiles of the longest request
     float c;                           // |scale| log2 e (1 when scale is 0)
-    float qmul;                        // sign of the scale (0 when it is 0): exact on any operand
+    uint32_t q_and, q_xor;             // the scale's sign on the queries' bits: their sign bits turned over (scale < 0), all bits cleared (scale 0)
 };
 
 // ---- LDS image of rows of RB bytes, 16-byte chunks XOR-swizzled so that 16 rows at one chunk, and 4 rows x 4 chunks, meet no bank twice ----
@@ -77,14 +79,12 @@ template <typename T, int D> struct Rows;
 
 template <int D> struct Rows<bf16, D> {
     bf16x8 q[D / 16];
-    DEVI void load(const bf16* p, bool ok, float mul, int lane) {
+    DEVI void load(const bf16* p, bool ok, const Args& a, int lane) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-            bf16x8 x = {};
-            if (ok) x = *reinterpret_cast<const bf16x8*>(p + 16 * s + 8 * (lane >> 5));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (bf16)((float)x[e] * mul);
-            q[s] = x;
+            u32x4 x = {};
+            if (ok) x = *reinterpret_cast<const u32x4*>(p + 16 * s + 8 * (lane >> 5));
+            q[s] = __builtin_bit_cast(bf16x8, (x & a.q_and) ^ (a.q_xor | a.q_xor >> 16));
         }
     }
     // scores of keys row0 .. + 32 of the image
@@ -123,12 +123,12 @@ template <int D> struct Rows<bf16, D> {
 // fp32: a step of v_mfma_f32_32x32x2_f32 takes one element per lane, lanes 0 - 31 of reduction slot 0 and lanes 32 - 63 of slot 1
 template <int D> struct Rows<float, D> {
     f32x4 q[D / 8];                                                // element (t, e) of half h: column 8 t + 4 h + e
-    DEVI void load(const float* p, bool ok, float mul, int lane) {
+    DEVI void load(const float* p, bool ok, const Args& a, int lane) {
 #pragma unroll
         for (int t = 0; t < D / 8; ++t) {
-            f32x4 x = {};
-            if (ok) x = *reinterpret_cast<const f32x4*>(p + 8 * t + 4 * (lane >> 5));
-            q[t] = x * mul;
+            u32x4 x = {};
+            if (ok) x = *reinterpret_cast<const u32x4*>(p + 8 * t + 4 * (lane >> 5));
+            q[t] = __builtin_bit_cast(f32x4, (x & a.q_and) ^ a.q_xor);
         }
     }
     DEVI f32x16 scores(const unsigned char* k, int row0, int lane) const {
@@ -243,24 +243,47 @@ DEVI int wave_upto(int v, int lane) {
     return v;
 }
 
-// `lds`: 3 (units + 1) ints; every wave ends with the same plan (the first one writes it)
+DEVI int wave_sum_int(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// `lds`: 3 (units + 1) ints; every wave ends with the same plan (the first one writes it).  Where nothing can be split (all lengths within the shortest run) there is
+// nothing to plan: item = (unit, tile of the longest request, head).
 template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     const int lane = threadIdx.x & 63;
     Plan p;
+    if (!a.split) {
+        p.run = 0x3fffffff;
+        p.items = a.units * a.tiles * a.d.kv_heads;
+        return p;
+    }
     p.item0 = lds;
     p.part0 = lds + a.units + 1;
     p.join0 = lds + 2 * (a.units + 1);
     int64_t work = 0;
-    bool odd = false;
     for (int u = lane; u < a.units; u += 64) {
         const Unit x = unit_of(a, u);
         work += (int64_t)tiles_of<TILE>(a, x) * x.kv;
-        odd |= x.n_all > a.d.max_q || x.kv != a.d.kv_lens[x.req / a.d.beams];
     }
-    if (odd) flag_page_error();
     work = wave_add(work) * a.d.kv_heads;
-    const int64_t run = (work + a.target - 1) / a.target;
-    p.run = (int)(max((int64_t)a.run_min, min(run, (int64_t)0x3fffffff)) + 63) / 64 * 64;
+    int64_t want = (work + a.target - 1) / a.target;
+    // steps: each request's last run is a short one; lengthen the runs until the workgroups that are resident together hold all of them
+#pragma unroll 1
+    for (int round = 0; round < (TILE == STEP_ROWS ? 4 : 1); ++round) {
+        p.run = (int)((max((int64_t)a.run_min, min(want, (int64_t)0x1fffffff)) + 63) / 64 * 64);
+        int n = 0, runs_most = 0;
+        for (int u = lane; u < a.units; u += 64) {
+            const Unit x = unit_of(a, u);
+            const int runs = max(1, (x.kv + p.run - 1) / p.run);
+            n += tiles_of<TILE>(a, x) * a.d.kv_heads * runs;
+            runs_most = max(runs_most, runs);
+        }
+        n = wave_sum_int(n);
+        if (n <= a.target || __ballot(runs_most > 1) == 0) break;
+        want = (int64_t)p.run * n / a.target + 1;
+    }
     int items = 0, parts = 0, joins = 0;
     for (int u0 = 0; u0 < a.units; u0 += 64) {
         const int u = u0 + lane;
@@ -294,6 +317,30 @@ DEVI int find(const int* first, int units, int i) {          // the last unit wh
     return lo;
 }
 
+// unit, run, tile and head of an item
+struct Item { int u, run, tile, head; Unit x; };
+template <int TILE> DEVI Item item_of(const Args& a, const Plan& plan, int item) {
+    Item it;
+    if (a.split) {
+        it.u = find(plan.item0, a.units, item);
+        it.x = unit_of(a, it.u);
+        int rest = item - plan.item0[it.u];
+        it.head = rest % a.d.kv_heads;
+        rest /= a.d.kv_heads;
+        const int tiles = tiles_of<TILE>(a, it.x);
+        it.tile = rest % tiles;
+        it.run = rest / tiles;
+    } else {
+        it.head = item % a.d.kv_heads;
+        it.tile = item / a.d.kv_heads % a.tiles;
+        it.u = item / a.d.kv_heads / a.tiles;
+        it.run = 0;
+        it.x = unit_of(a, it.u);
+    }
+    if (it.tile == 0 && it.run == 0 && it.head == 0 && threadIdx.x == 0 && (it.x.n_all > a.d.max_q || it.x.kv != a.d.kv_lens[it.x.req / a.d.beams])) flag_page_error();
+    return it;
+}
+
 // a row of a unit: beam, token, query head within the group -> its token row, or -1 where it has none
 struct Row { int64_t token; int head, beam, i; };
 DEVI Row row_of(const Args& a, const Unit& x, int row) {
@@ -324,7 +371,6 @@ DEVI void store4(float* p, float a, float b, float c, float d) { *reinterpret_ca
 // ------------------------------------------------------------------------------------------------
 // chunks
 // ------------------------------------------------------------------------------------------------
-constexpr int CHUNK_ROWS = 128;
 template <typename T> constexpr int chunk_subtiles = sizeof(T) == 2 ? 2 : 1;      // 64 keys a tile in bf16, 32 in fp32: 32 or 16 KB of K and V at head_dim 64 or 128 either way
 template <typename T, int D> constexpr int chunk_lds = 2 * 2 * 32 * chunk_subtiles<T> * D * (int)sizeof(T);
 
@@ -335,12 +381,10 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Plan plan = make_plan<CHUNK_ROWS>(a, reinterpret_cast<int*>(lds + 4 * IMG));
     for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
-        const int u = find(plan.item0, a.units, item);
-        const Unit x = unit_of(a, u);
-        int rest = item - plan.item0[u];
-        const int h = rest % a.d.kv_heads;
-        rest /= a.d.kv_heads;
-        const int tiles = tiles_of<CHUNK_ROWS>(a, x), tile = rest % tiles, run = rest / tiles, row0 = tile * CHUNK_ROWS;
+        const Item it = item_of<CHUNK_ROWS>(a, plan, item);
+        const Unit& x = it.x;
+        const int u = it.u, h = it.head, run = it.run, row0 = it.tile * CHUNK_ROWS;
+        if (row0 >= x.n * a.group) continue;                                     // (a tile that only the longest request has)
         const bool whole = plan.run >= x.kv;
         const int last = min(x.n * a.group, row0 + CHUNK_ROWS) - 1;
         const int end = min(sees(a, x, last / a.group), (run + 1) * plan.run);
@@ -348,7 +392,7 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         const Row row = row_of(a, x, row0 + 32 * wave + (lane & 31));
         const int lim = row.token >= 0 ? sees(a, x, row.i) : 0x7fffffff;      // (rows without a token compute on zeros: nothing of them is written)
         Rows<T, D> rows;
-        rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a.qmul, lane);
+        rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a, lane);
         int free_to = lim;                                                       // keys every row of the wave sees
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) free_to = min(free_to, __shfl_xor(free_to, o, 64));
@@ -404,72 +448,90 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
 // ------------------------------------------------------------------------------------------------
 // steps
 // ------------------------------------------------------------------------------------------------
-constexpr int STEP_ROWS = 32;
-template <typename T, int D> constexpr int step_lds = 4 * 2 * 32 * D * (int)sizeof(T);       // a tile of 32 keys per wave
+template <typename T, int D> constexpr int step_buffers = D * (int)sizeof(T) <= 128 ? 2 : 1;
+template <typename T, int D> constexpr int step_lds = step_buffers<T, D> * 4 * 2 * 32 * D * (int)sizeof(T);       // one or two tiles of 32 keys per wave
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_attn_step_kernel(Args a) {
     extern __shared__ unsigned char lds[];
-    constexpr int RB = D * (int)sizeof(T), IMG = 32 * RB;
+    constexpr int RB = D * (int)sizeof(T), IMG = 32 * RB, BUF = step_buffers<T, D>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned char* mine = lds + wave * 2 * IMG;
-    int* shared_to = reinterpret_cast<int*>(lds + 8 * IMG);
+    unsigned char* mine = lds + wave * BUF * 2 * IMG;
+    int* shared_to = reinterpret_cast<int*>(lds + BUF * 8 * IMG);
     const Plan plan = make_plan<STEP_ROWS>(a, shared_to + 4);
     for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
-        const int u = find(plan.item0, a.units, item);
-        const Unit x = unit_of(a, u);
-        const int h = (item - plan.item0[u]) % a.d.kv_heads, run = (item - plan.item0[u]) / a.d.kv_heads;
+        const Item it = item_of<STEP_ROWS>(a, plan, item);
+        const Unit& x = it.x;
+        const int u = it.u, h = it.head, run = it.run;
+        if (x.n == 0) continue;
         const int start = run * plan.run, end = min(x.kv, start + plan.run);
         const bool whole = plan.run >= x.kv;
         const int n_rows = x.nb * x.n * a.group;
         const Row row = row_of(a, x, lane & 31);
-        const int lim = row.token >= 0 ? min(sees(a, x, row.i), end) : 0x7fffffff;
+        const int lim = row.token >= 0 ? sees(a, x, row.i) : 0x7fffffff;
         Rows<T, D> rows;
-        rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a.qmul, lane);
+        rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a, lane);
         int free_to = lim;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) free_to = min(free_to, __shfl_xor(free_to, o, 64));
         const int32_t* table = a.d.tables + x.req * a.d.table_row;
         const int64_t head_off = h * a.d.head_stride;
-        // whole tiles whose pages are the same for every beam are read once for all of them: blocks up to the first that differs
+        // pages that are the same for every beam are read once for all of them: up to the first block that differs
         __syncthreads();                                                         // the item before has read shared_to and the tiles
-        int shared_tiles = (max(end - start, 0) + 31) / 32;
+        int shared_end = max(end, start);
         if (x.nb > 1 && end > start) {
             int differs = 0x7fffffff;
             const int b1 = (end - 1) >> a.page_shift;
             for (int b = (start >> a.page_shift) + threadIdx.x; b <= b1; b += 256) {
                 const int p = table[b];
-                for (int w = 1; w < x.nb; ++w)
-                    if (table[w * a.d.table_row + b] != p) differs = min(differs, b);
+                bool same = true;
+#pragma unroll 4
+                for (int w = 1; w < x.nb; ++w) same &= table[w * a.d.table_row + b] == p;
+                if (!same) differs = min(differs, b);
             }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) differs = min(differs, __shfl_xor(differs, o, 64));
             if (lane == 0) shared_to[wave] = differs;
             __syncthreads();
             differs = min(min(shared_to[0], shared_to[1]), min(shared_to[2], shared_to[3]));
-            if (differs <= b1) shared_tiles = max(0, (int)(((int64_t)differs << a.page_shift) - start)) / 32;
+            if (differs <= b1) shared_end = max(start, differs << a.page_shift);
         }
-        const int tiles = (max(end - start, 0) + 31) / 32, jobs = shared_tiles + (tiles - shared_tiles) * x.nb;
+        // jobs: the shared tiles, then each beam's own
+        const int shared_tiles = (shared_end - start + 31) / 32, jobs = shared_tiles + (max(end - shared_end, 0) + 31) / 32 * x.nb;
+        struct Job { int key0, end, beam; };
+        auto job = [&](int j) {
+            const int k = j - shared_tiles;
+            return k < 0 ? Job{start + 32 * j, shared_end, -1} : Job{shared_end + 32 * (k / x.nb), j < jobs ? end : 0, k % x.nb};
+        };
+        auto pages = [&](const Job& b) { return page_of<32>(a, table + max(b.beam, 0) * a.d.table_row, b.key0, b.end, lane); };
         float m = -INFINITY, l = 0.f;
         f32x16 o[D / 32] = {};
-        auto job = [&](int j, int& key0, int& w) {
-            const bool one = j >= shared_tiles;
-            key0 = start + 32 * (one ? shared_tiles + (j - shared_tiles) / x.nb : j);
-            w = one ? (j - shared_tiles) % x.nb : -1;
-            return page_of<32>(a, table + max(w, 0) * a.d.table_row, key0, j < jobs ? end : 0, lane);
-        };
-        int key0, w, page = job(wave, key0, w);
+        Job now = job(wave), next = job(wave + 4);
+        int page_now = pages(now), page_next = pages(next);
+        constexpr int LOADS = 2 * 32 * RB / 1024;                                // LDS-DMA instructions of a tile
+        if (BUF == 2 && wave < jobs) stage<T, D, 32, 1>(a, now.key0, now.end, page_now, head_off, mine, mine + IMG, 0, lane);
         for (int j = wave; j < jobs; j += 4) {
-            const int key0_now = key0, w_now = w;
-            stage<T, D, 32, 1>(a, key0, end, page, head_off, mine, mine + IMG, 0, lane);
-            page = job(j + 4, key0, w);                                          // (the next tile's pages come along with this tile)
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (w_now < 0) tile_step<T, D, 1>(rows, mine, mine + IMG, key0_now, lim, key0_now + 32 > free_to, a.c, m, l, o, lane);
-            else {                                                               // a tile of one beam: the other beams' rows see none of it
-                const bool take = row.beam == w_now;
-                tile_step<T, D, 1, true>(rows, mine, mine + IMG, key0_now, take ? lim : 0, true, a.c, m, l, o, lane, take);
+            unsigned char* img = mine + (BUF == 2 ? ((j >> 2) & 1) * 2 * IMG : 0);
+            const Job after = job(j + 8);
+            const int page_after = pages(after);                                 // (older than the loads of the next tile: waiting for it leaves those in flight)
+            if (BUF == 2) {
+                if (j + 4 < jobs) {
+                    unsigned char* to = mine + (((j >> 2) + 1) & 1) * 2 * IMG;
+                    stage<T, D, 32, 1>(a, next.key0, next.end, page_next, head_off, to, to + IMG, 0, lane);
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");  // this tile's loads are older than the last LOADS
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+            } else {
+                stage<T, D, 32, 1>(a, now.key0, now.end, page_now, head_off, img, img + IMG, 0, lane);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
+            const int see = min(lim, now.end);
+            const bool take = now.beam < 0 || row.beam == now.beam;              // a tile of one beam: the other beams' rows see none of it
+            tile_step<T, D, 1, true>(rows, img, img + IMG, now.key0, take ? see : 0, now.beam >= 0 || now.key0 + 32 > min(free_to, now.end), a.c, m, l, o, lane, take);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                   // the tile is read before the next one lands on it
+            now = next; next = after;
+            page_now = page_next; page_next = page_after;
         }
         l += other_half(l);
         // the four waves' sums meet: [wave][row][D] fp32 in the tiles' place, [wave][row][2] behind
@@ -538,16 +600,27 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(Args a) {
         if (row.token < 0) continue;
         float top = -INFINITY, den = 0.f;
         f32x4 sum = {};
-        for (int r = 0; r < runs; ++r) {
-            const int part = plan.part0[u] + (r * tiles + tile) * a.d.kv_heads + h;
-            const float* ml = part_ml<D, TILE>(a, part) + 2 * at_row;
-            const float mr = ml[0], lr = ml[1];
-            const f32x4 v = *reinterpret_cast<const f32x4*>(part_o<D, TILE>(a, part) + at_row * D + e);
-            const float next = fmaxf(top, mr), mm = next == -INFINITY ? 0.f : next;
-            const float fa = __builtin_amdgcn_exp2f(top - mm), fb = __builtin_amdgcn_exp2f(mr - mm);
-            den = den * fa + lr * fb;
-            sum = sum * fa + v * fb;
-            top = next;
+        constexpr int AT_ONCE = 8;
+        for (int r0 = 0; r0 < runs; r0 += AT_ONCE) {                             // loads of eight runs in flight
+            float mr[AT_ONCE], lr[AT_ONCE];
+            f32x4 v[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int part = plan.part0[u] + (min(r0 + k, runs - 1) * tiles + tile) * a.d.kv_heads + h;
+                const float* ml = part_ml<D, TILE>(a, part) + 2 * at_row;
+                mr[k] = ml[0];
+                lr[k] = ml[1];
+                v[k] = *reinterpret_cast<const f32x4*>(part_o<D, TILE>(a, part) + at_row * D + e);
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                if (r0 + k >= runs) continue;
+                const float next = fmaxf(top, mr[k]), mm = next == -INFINITY ? 0.f : next;
+                const float fa = __builtin_amdgcn_exp2f(top - mm), fb = __builtin_amdgcn_exp2f(mr[k] - mm);
+                den = den * fa + lr[k] * fb;
+                sum = sum * fa + v[k] * fb;
+                top = next;
+            }
         }
         const float inv = den != 0.f ? 1.f / den : 0.f;
         store4(out_row<T, D>(a, row, h) + e, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
@@ -560,7 +633,7 @@ Shape shape_of(const mmf_paged_attn_desc* d) {
     const int64_t rows = (int64_t)d->max_q * (d->heads / d->kv_heads);
     s.chunk = rows > STEP_ROWS;
     s.nb = s.chunk ? 1 : (int)(STEP_ROWS / rows < d->beams ? STEP_ROWS / rows : d->beams);
-    s.target = 1024;
+    s.target = s.chunk ? 1024 : 512;
     s.run_min = s.chunk ? 1024 : 256;
     s.split = (int64_t)d->blocks * d->page_size > s.run_min;
     s.ws = s.split ? (int64_t)2 * s.target * (s.chunk ? CHUNK_ROWS : STEP_ROWS) * (d->head_dim + 2) * 4 : 0;
@@ -586,9 +659,12 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
     a.nb = s.nb;
     a.per_group = (d->beams + s.nb - 1) / s.nb;
     a.target = s.target;
-    a.run_min = s.split ? s.run_min : 0x3fffffff;
+    a.run_min = s.run_min;
+    a.split = s.split;
+    a.tiles = s.chunk ? (int)(((int64_t)d->max_q * a.group + CHUNK_ROWS - 1) / CHUNK_ROWS) : 1;
     a.c = d->scale != 0.f ? fabsf(d->scale) * 1.44269504088896340736f : 1.f;
-    a.qmul = d->scale > 0.f ? 1.f : d->scale < 0.f ? -1.f : 0.f;
+    a.q_and = d->scale != 0.f ? 0xffffffffu : 0u;
+    a.q_xor = d->scale < 0.f ? 0x80000000u : 0u;
     const int step = UNITS_MAX / a.per_group * d->beams;         // requests per launch: whole groups
     for (int r0 = 0; r0 < d->requests; r0 += step) {
         const int n = d->requests - r0 < step ? d->requests - r0 : step;
@@ -599,9 +675,9 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
         a.d.q_start = d->q_start + r0;
         a.units = s.nb == 1 ? n : n / d->beams * a.per_group;
         const int prefix = 3 * (a.units + 1) * 4;
-        const int64_t tiles = s.chunk ? ((int64_t)d->max_q * a.group + CHUNK_ROWS - 1) / CHUNK_ROWS : 1;
-        int64_t most = tiles * a.units * d->kv_heads + (s.split ? 2 * s.target : 0);
-        const int grid = (int)(most < s.target ? most : s.target);
+        const int64_t most = (int64_t)a.tiles * a.units * d->kv_heads;
+        MMF_CHECK_ARG(most <= 0x3fffffff, "paged_attention: too many rows for one call");
+        const int grid = s.split || most > s.target ? s.target : (int)most;
         if (s.chunk) {
             const int lds = chunk_lds<T, D> + prefix;
             static std::atomic<uint64_t> done{0};
