@@ -48,19 +48,23 @@ constexpr int PLAN_THREADS = 1024;       // (256 where that is a thread per grou
 DEVI int blocks_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
 // Pages of released groups, back on the stack in the order of their rows and blocks; returns the new top.  A wave counts a row's pages, the counts are scanned,
-// a wave pushes them; `counts` holds one int per row.
-DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, int* counts, int64_t* lds) {
+// a wave pushes them; `counts` holds one int per row, `list` another: the rows to release, in any order.
+DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, int* counts, int* list, int* released, int64_t* lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6, R = d.groups * d.beams;
+    for (int r = tid; r < R; r += blockDim.x) {
+        counts[r] = 0;
+        if (d.q_lens[r / d.beams] < 0) list[atomicAdd(released, 1)] = r;
+    }
+    __syncthreads();
+    const int n_list = *released;
 #pragma unroll 1
-    for (int r = wave; r < R; r += waves) {
+    for (int k = wave; k < n_list; k += waves) {
         int n = 0;
-        const int g = r / d.beams;
-        if (d.q_lens[g] < 0) {
-            const int blocks = min(blocks_of(max(d.kv_lens[g], 0), shift), d.blocks);
-            for (int j = lane; j < blocks; j += 64) n += d.owned[(size_t)r * d.blocks + j] >= 0;
+        const int r = list[k], blocks = min(blocks_of(max(d.kv_lens[r / d.beams], 0), shift), d.blocks);
+#pragma unroll 4
+        for (int j = lane; j < blocks; j += 64) n += d.owned[(size_t)r * d.blocks + j] >= 0;
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-        }
+        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
         if (lane == 0) counts[r] = n;
     }
     __syncthreads();
@@ -74,7 +78,8 @@ DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, int* cou
     }
     __syncthreads();
 #pragma unroll 1
-    for (int r = wave; r < R; r += waves) {
+    for (int k = wave; k < n_list; k += waves) {
+        const int r = list[k];
         int at = counts[r];
         if (at < 0) continue;
         const int blocks = min(blocks_of(max(d.kv_lens[r / d.beams], 0), shift), d.blocks);
@@ -128,14 +133,14 @@ DEVI void plan_row(const mmf_paged_plan_desc& d, int shift, const PlanGroup& g, 
     }
 }
 
-// rows_too: a row by one thread, or by eight where some have more than four tokens; else the second launch takes a wave per row
+// rows_too: a row by one thread, or by eight where some have more than four tokens; else the second launch takes workgroups for each
 __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc d, int shift, int rows_too) {
     __shared__ int64_t lds[PLAN_THREADS / 64];
-    __shared__ int taken, refused, flags;                         // flags: 1 a group is released, 2 a row has many tokens
+    __shared__ int taken, refused, flags, released;               // flags: 1 a group is released, 2 a row has many tokens
     const int tid = threadIdx.x, threads = blockDim.x, W = d.beams, per = d.shared ? 1 : W;
     PlanGroup* ws = reinterpret_cast<PlanGroup*>(d.ws);
-    int* tail = reinterpret_cast<int*>(ws + d.groups);             // [0]: the top the pages are taken from, [4 ..]: plan_release's counts
-    if (tid == 0) { taken = 0; refused = 0; flags = 0; }
+    int* tail = reinterpret_cast<int*>(ws + d.groups);             // [0]: the top the pages are taken from, [4 ..]: plan_release's counts and list
+    if (tid == 0) { taken = 0; refused = 0; flags = 0; released = 0; }
     for (int i = tid; i < 3 * d.groups * W; i += threads) d.copies[i] = -1;
     const int told = d.free_top[0];
     int top = min(max(told, 0), d.free_capacity);
@@ -150,7 +155,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc 
     const int f = (least < 0) | (most > 4) << 1;
     if (f) atomicOr(&flags, f);
     __syncthreads();
-    if (flags & 1) top = plan_release(d, shift, top, tail + 4, lds);
+    if (flags & 1) top = plan_release(d, shift, top, tail + 4, tail + 4 + d.groups * W, &released, lds);
     const int per_row = flags & 2 ? 8 : 1;
     int carry_need = 0, total;
     int64_t carry_rows = 0, total64;
@@ -199,10 +204,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc 
 }
 __global__ __launch_bounds__(256) void plan_rows_kernel(mmf_paged_plan_desc d, int shift) {
     const PlanGroup* ws = reinterpret_cast<const PlanGroup*>(d.ws);
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= d.groups * d.beams) return;
-    const int g = r / d.beams;
-    plan_row(d, shift, ws[g], r, r - g * d.beams, d.shared ? d.q_start[g] : d.q_start[r], reinterpret_cast<const int*>(ws + d.groups)[0], threadIdx.x & 63, 64);
+    const int r = blockIdx.x, g = r / d.beams;
+    plan_row(d, shift, ws[g], r, r - g * d.beams, d.shared ? d.q_start[g] : d.q_start[r], reinterpret_cast<const int*>(ws + d.groups)[0],
+             blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -276,7 +280,7 @@ DEVI double log_of(double x) {
     return 2.0 * s * p + e * 0.69314718055994530942;
 }
 
-// 16 bytes of a row as floats, NaN as -inf; WIDE: rows start on 4 bytes, else on an element
+// 16 bytes of a row as floats; WIDE: rows start on 4 bytes, else on an element.  (NaN loses every comparison and maximum below, as -inf does.)
 template <typename T, bool WIDE> struct Reader {
     static constexpr int VEC = 16 / (int)sizeof(T);
     typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(4)));
@@ -290,10 +294,7 @@ template <typename T, bool WIDE> struct Reader {
             for (int e = 0; e < VEC; ++e) raw[e] = at + e < n ? x[at + e] : (T)-INFINITY;
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float f = (float)raw[e];
-            v[e] = f == f ? f : -INFINITY;
-        }
+        for (int e = 0; e < VEC; ++e) v[e] = (float)raw[e];
     }
 };
 
@@ -326,7 +327,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(mmf_beam_select_desc d, 
     const float bar = fmaxf(fmaxf(bars[0], bars[1]), fmaxf(bars[2], bars[3]));
     const float base = top > -INFINITY && top < INFINITY ? top : 0.f;
     double s = 0.0;
-#pragma unroll 1
+#pragma unroll 2
     for (int at = tid * VEC; at < n; at += 256 * VEC) {
         float v[VEC];
         R::load(x, at, n, v);
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(mmf_beam_select_desc d, 
         int bi = 0x7fffffff;
 #pragma unroll 1
         for (int i = tid; i < n; i += 256) {
-            const float f = (float)x[i], y = f == f ? f : -INFINITY;
+            const float y = (float)x[i];
             if (y > -INFINITY && (y < last || (y == last && i > last_i)) && (y > bv || (y == bv && i < bi))) { bv = y; bi = i; }
         }
 #pragma unroll
@@ -531,16 +532,19 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     __syncthreads();
     if (!d.history) return;
     const int64_t at = (int64_t)g * W * d.length;
-    constexpr int COLS = 32;                                      // through LDS, 32 columns at a time: in place as well
-    for (int64_t t0 = 0; t0 < d.length; t0 += COLS) {
-        for (int k = tid; k < W * COLS; k += 256) {
-            const int w = k / COLS;
-            const int64_t t = t0 + k % COLS;
+    const int cols = LIST / W;                                    // through LDS, many columns at a time: in place as well
+    for (int64_t t0 = 0; t0 < d.length; t0 += cols) {
+        for (int k = tid; k < W * cols; k += 256) {
+            const int w = k / cols;
+            const int64_t t = t0 + k - w * cols;
             if (t < d.length) cand_i[k] = t == d.step ? best_i[w] : d.history[at + parent[w] * d.length + t];
         }
         __syncthreads();
-        for (int k = tid; k < W * COLS; k += 256)
-            if (t0 + k % COLS < d.length) d.history_out[at + k / COLS * d.length + t0 + k % COLS] = cand_i[k];
+        for (int k = tid; k < W * cols; k += 256) {
+            const int w = k / cols;
+            const int64_t t = t0 + k - w * cols;
+            if (t < d.length) d.history_out[at + w * d.length + t] = cand_i[k];
+        }
         __syncthreads();
     }
 }
@@ -561,6 +565,7 @@ int beam_segments(int rows, int64_t vocab, int* length) {
 // no child, of which there are exactly as many, and get its tokens copied.  A page that is copied from is never copied to.
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void reorder_tables_kernel(mmf_paged_reorder_desc d) {
+    __shared__ int pages[LIST], copied[MMF_BEAMS_MAX];
     __shared__ int parent[MMF_BEAMS_MAX], source[MMF_BEAMS_MAX];  // source[w]: the beam whose last page beam w goes on writing
     const int g = blockIdx.x, tid = threadIdx.x, W = d.beams;
     if (tid < W) {
@@ -579,19 +584,28 @@ __global__ __launch_bounds__(256) void reorder_tables_kernel(mmf_paged_reorder_d
         }
     }
     __syncthreads();
-    const int kv = max(d.kv_lens[g], 0), part = kv % d.page_size ? kv / d.page_size : -1;
-    for (int j = tid; j < d.blocks; j += 256) {                   // a column at a time: in place as well
-        int t[MMF_BEAMS_MAX];
-        for (int w = 0; w < W; ++w) t[w] = d.tables[((size_t)g * W + w) * d.blocks + j];
-        for (int w = 0; w < W; ++w) d.tables_out[((size_t)g * W + w) * d.blocks + j] = t[j == part ? source[w] : parent[w]];
-        if (j == part)
-            for (int w = 0; w < W; ++w) {
-                const bool copy = source[w] != parent[w];
-                int* c = d.copies + 3 * ((size_t)g * W + w);
-                c[0] = copy ? t[parent[w]] : -1;
-                c[1] = copy ? t[source[w]] : -1;
-                c[2] = copy ? kv % d.page_size : -1;
-            }
+    const int kv = max(d.kv_lens[g], 0), rest = kv & (d.page_size - 1), part = rest ? kv / d.page_size : -1, cols = LIST / W;
+    const int* from = d.tables + (size_t)g * W * d.blocks;
+    int* to = d.tables_out + (size_t)g * W * d.blocks;
+    for (int j0 = 0; j0 < d.blocks; j0 += cols) {                 // through LDS, many columns at a time: in place as well
+        for (int k = tid; k < W * cols; k += 256) {
+            const int w = k / cols, j = j0 + k - w * cols;
+            if (j < d.blocks) pages[k] = from[(size_t)(j == part ? source[w] : parent[w]) * d.blocks + j];
+        }
+        if (part >= j0 && part < j0 + cols && part < d.blocks && tid < W) copied[tid] = source[tid] != parent[tid] ? from[(size_t)parent[tid] * d.blocks + part] : -1;
+        __syncthreads();
+        for (int k = tid; k < W * cols; k += 256) {
+            const int w = k / cols, j = j0 + k - w * cols;
+            if (j < d.blocks) to[(size_t)w * d.blocks + j] = pages[k];
+        }
+        if (part >= j0 && part < j0 + cols && part < d.blocks && tid < W) {
+            int* c = d.copies + 3 * ((size_t)g * W + tid);
+            const bool copy = source[tid] != parent[tid];
+            c[0] = copied[tid];
+            c[1] = copy ? pages[tid * cols + part - j0] : -1;
+            c[2] = copy ? rest : -1;
+        }
+        __syncthreads();
     }
     if ((part < 0 || part >= d.blocks) && tid < 3 * W) d.copies[3 * (size_t)g * W + tid] = -1;
 }
@@ -606,13 +620,18 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(mmf_paged_copy_desc d, 
         if (threadIdx.x == 0 && blockIdx.y == 0) flag_page_error();
         return;
     }
-    const int per_pos = d.head_dim * esize / (int)sizeof(VT), n = d.kv_heads * tokens * per_pos;
     char* base = (char*)d.cache + blockIdx.y * d.plane_stride * esize;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int h = i / (tokens * per_pos), k = i - h * tokens * per_pos, pos = k / per_pos, e = (k - pos * per_pos) * (int)sizeof(VT);
-        const int64_t off = (h * d.head_stride + pos * d.pos_stride) * esize + e;
-        *reinterpret_cast<VT*>(base + dst * d.page_stride * esize + off) = *reinterpret_cast<const VT*>(base + src * d.page_stride * esize + off);
-    }
+    char* to = base + dst * d.page_stride * esize;
+    const char* from = base + src * d.page_stride * esize;
+    const int per_pos = d.head_dim * esize / (int)sizeof(VT), n = tokens * per_pos, lane = threadIdx.x & 63;
+    const bool dense = d.pos_stride == d.head_dim;
+    for (int h = threadIdx.x >> 6; h < d.kv_heads; h += 4)        // a wave per head
+#pragma unroll 4
+        for (int i = lane; i < n; i += 64) {
+            const int pos = dense ? 0 : i / per_pos;
+            const int64_t off = (h * d.head_stride + pos * d.pos_stride) * esize + (int64_t)(i - pos * per_pos) * (int)sizeof(VT);
+            *reinterpret_cast<VT*>(to + off) = *reinterpret_cast<const VT*>(from + off);
+        }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -629,7 +648,7 @@ int mmf_decode_take_error(void) {
 }
 
 int64_t mmf_paged_plan_ws_bytes(int groups, int beams) {
-    return groups > 0 && beams > 0 ? (int64_t)groups * (int64_t)sizeof(PlanGroup) + 16 + 4 * (int64_t)groups * beams : 0;
+    return groups > 0 && beams > 0 ? (int64_t)groups * (int64_t)sizeof(PlanGroup) + 16 + 8 * (int64_t)groups * beams : 0;
 }
 
 int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream) {
@@ -645,8 +664,10 @@ int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream) {
     const int shift = __builtin_ctz(d->page_size);
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(rows <= 256 ? 256 : PLAN_THREADS), 0, (hipStream_t)stream, *d, shift, (int)one);
     MMF_CHECK_LAUNCH();
-    if (!one) {
-        hipLaunchKernelGGL(plan_rows_kernel, dim3((d->groups * d->beams + 3) / 4), dim3(256), 0, (hipStream_t)stream, *d, shift);
+    if (!one) {                                                   // a workgroup per row, and a few where rows have many tokens on average: some have many times that
+        const int64_t wide = d->rows / rows / 64;
+        const unsigned y = (unsigned)(wide < 1 ? 1 : wide > 8 ? 8 : wide);
+        hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)rows, y), dim3(256), 0, (hipStream_t)stream, *d, shift);
         MMF_CHECK_LAUNCH();
     }
     return 0;
@@ -700,7 +721,7 @@ int mmf_beam_select(const mmf_beam_select_desc* d, void* stream) {
 int mmf_paged_reorder(const mmf_paged_reorder_desc* d, void* stream) {
     MMF_CHECK_ARG(d && d->parents && d->kv_lens && d->tables && d->tables_out && d->copies, "paged_reorder: null operand");
     MMF_CHECK_ARG(d->groups > 0 && d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->blocks > 0, "paged_reorder: bad shape");
-    MMF_CHECK_ARG(d->page_size >= 1 && d->page_size <= MMF_PAGE_MAX, "paged_reorder: bad page_size");
+    MMF_CHECK_ARG(d->page_size >= 1 && d->page_size <= MMF_PAGE_MAX && (d->page_size & (d->page_size - 1)) == 0, "paged_reorder: page_size is a power of two up to 1024");
     hipLaunchKernelGGL(reorder_tables_kernel, dim3(d->groups), dim3(256), 0, (hipStream_t)stream, *d);
     MMF_CHECK_LAUNCH();
     return 0;
