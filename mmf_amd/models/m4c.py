@@ -16,6 +16,7 @@ On the device:
     row, which one MFMA GEMM (zero-padded to 3008 columns) projects;
   * `_batch_gather(cat([ans_emb, ocr_emb]))` is a two-source row gather (no [B, 5050, 768] concatenation);
   * classifier GEMM and pointer-network kernel write the two halves of the [B, T, 5000 + 50] score tensor in place;
+  * with `num_beams` in the model's config, evaluation decodes by beam search over a paged key / value cache (mmf_amd/decoding.py);
   * greedy decoding (:290-305) re-runs only the multimodal transformer per step: `text_bert` is deterministic in eval
     mode, so its output is computed once instead of `dec_step_num` times.
 
@@ -27,6 +28,7 @@ import warnings
 import torch
 from torch import nn
 
+from mmf_amd import _native as nat
 from mmf_amd import functional as Fn
 from mmf_amd import fp32_path as F32P
 from mmf_amd import fp32_train as F32T
@@ -310,7 +312,7 @@ class M4C(BaseModel):
         self._forward_obj_encoding(sample_list, fwd_results)
         self._forward_ocr_encoding(sample_list, fwd_results)
         self._forward_mmt_and_output(sample_list, fwd_results)
-        return {"scores": fwd_results["scores"]}
+        return {k: fwd_results[k] for k in ("scores", "beam_tokens", "beam_scores") if k in fwd_results}
 
     def _forward_txt_encoding(self, sample_list, fwd_results):
         fwd_results["txt_inds"] = sample_list["text"]
@@ -397,6 +399,8 @@ class M4C(BaseModel):
             fwd_results["prev_inds"] = sample_list["train_prev_inds"].clone()
             self._forward_mmt(sample_list, fwd_results)
             self._forward_output(sample_list, fwd_results)
+        elif self.config.get("num_beams", 0):
+            self._decode_beams(sample_list, fwd_results, int(self.config.num_beams))
         elif self.config.get("kv_cached_decode", True) and not F32P.active() and not F32T.active():
             self._decode_incremental(sample_list, fwd_results)
         else:
@@ -465,6 +469,98 @@ class M4C(BaseModel):
             if i + 1 < D:
                 prev[:, i + 1] = s_i[:, 0].argmax(dim=-1)
         fwd_results["scores"] = scores
+        fwd_results["prev_inds"] = prev
+        fwd_results["mmt_ocr_output"] = mmt_ocr_output
+
+    @torch.no_grad()
+    def _decode_beams(self, sample_list, fwd_results, W):
+        """Beam search with `num_beams` beams instead of the greedy loop (m4c.py:290-305), through mmf_amd.decoding: the valid encoder positions of a sample go
+        through the multimodal transformer once, packed, into pages that its beams share; a step runs one row per beam, selects over beams x (vocabulary + OCR
+        tokens) by the sum of log-probabilities (the reference's BeamSearch, mmf/utils/text.py), and reorders the pages after the parents.  A beam that has
+        produced the end token keeps its score.  Leaves `beam_tokens` [B, W, D] and `beam_scores` [B, W], best first, and as `scores` [B, D, V + N] the score rows along the best
+        beam.  bf16, or fp32 inside `mmf_amd.fp32_inference()`."""
+        from mmf_amd import decoding
+        from mmf_amd.modules.infer import layer_rows_paged
+        if F32T.active():
+            raise NotImplementedError("num_beams decodes on the bf16 path or inside mmf_amd.fp32_inference()")
+        f32 = F32P.active()
+        if "txt_emb" not in fwd_results:
+            fwd_results["txt_emb"] = self.text_bert_out_linear(self.text_bert(txt_inds=fwd_results["txt_inds"], txt_mask=fwd_results["txt_mask"]))
+        txt_emb, obj_emb, ocr_emb = fwd_results["txt_emb"], fwd_results["obj_mmt_in"], fwd_results["ocr_mmt_in"]
+        ocr_mask = fwd_results["ocr_mask"]
+        B, T, H = txt_emb.shape
+        O, N = obj_emb.shape[1], ocr_emb.shape[1]
+        D, E = sample_list["train_prev_inds"].size(1), T + O + N
+        dev, dtype = txt_emb.device, torch.float32 if f32 else torch.bfloat16
+        layers = self.mmt.encoder.layer
+        heads = layers[0].attention.self.num_attention_heads
+
+        # the valid positions of all samples, one after another; the others follow behind
+        valid = torch.cat([fwd_results["txt_mask"], fwd_results["obj_mask"], ocr_mask], dim=1) > 0
+        order = torch.sort((~valid).flatten().to(torch.int8), stable=True).indices
+        back = torch.empty_like(order)
+        back[order] = torch.arange(B * E, device=dev)
+        gather = nat.gather_rows2_f32 if f32 else nat.gather_rows2
+
+        def rows(x, index):
+            out = torch.empty(B * E, H, dtype=dtype, device=dev)
+            gather(x, x, index, out, B * E, H)
+            return out
+
+        cache = decoding.PagedCache(len(layers), B, W, E + D, kv_heads=heads, head_dim=H // heads, dtype=dtype, device=dev)
+        plan = cache.plan(valid.sum(1, dtype=torch.int32), B * E, shared=True)
+        concat = F32P.concat_rows if f32 else Fn.ConcatRowsFn.apply
+        x = rows(concat(txt_emb, obj_emb, ocr_emb).reshape(B * E, H), order)
+        ctxt = torch.zeros(B * E, heads, H // heads, dtype=dtype, device=dev)       # (positions that are padding attend to nothing)
+        for l, layer in enumerate(layers):
+            x = layer_rows_paged(layer, x, cache, l, plan, E, False, out_rows=ctxt)
+        mmt_ocr_output = rows(x, back).view(B, E, H)[:, T + O:].contiguous()
+
+        pp, cls, ptr = self.mmt.prev_pred_embeddings, self.classifier.module, self.ocr_ptr_net
+        V = cls.weight.shape[0]
+        ans_emb = pp.ans_layer_norm(cls.weight.detach() if f32 else Fn.ParamRowsFn.apply(cls.weight))
+        ocr_ln = pp.ocr_layer_norm(ocr_emb)
+        zero = torch.zeros(B * W, 1, H, dtype=dtype, device=dev)
+        ocr_mask_add = _additive(ocr_mask)
+        X = F32P if f32 else None
+        ones = torch.ones(B, dtype=torch.int32, device=dev)
+        eos = int(self.answer_processor.get("EOS_IDX", 2) if hasattr(self.answer_processor, "get") else getattr(self.answer_processor, "EOS_IDX", 2))
+        tokens = torch.full((B, W), int(self.answer_processor.BOS_IDX), dtype=torch.long, device=dev)
+        scores = torch.full((B, W), float("-inf"), device=dev)
+        scores[:, 0] = 0.0
+        beams = decoding.BeamStep(scores, None, None, torch.zeros(B, W, dtype=torch.bool, device=dev), torch.zeros(B, W, D, dtype=torch.long, device=dev))
+        seen, parents = [], []
+        for i in range(D):
+            plan = cache.plan(ones, B * W)
+            raw = (X.prev_pred_gather if X else Fn.PrevPredGatherFn.apply)(ans_emb, ocr_ln, tokens)
+            emb = (X.add_pos_type if X else Fn.AddPosTypeFn.apply)(zero, tokens.ge(V).long().view(B * W, 1), pp.position_embeddings.weight[i:i + 1],
+                                                                   pp.token_type_embeddings.weight)
+            x = (X.add if X else Fn.AddFn.apply)(raw.reshape(B * W, H), pp.emb_layer_norm(emb).reshape(B * W, H))
+            for l, layer in enumerate(layers):
+                x = layer_rows_paged(layer, x, cache, l, plan, 1, True)
+            if f32:
+                s = F32P.m4c_scores(x.view(B, W, H), mmt_ocr_output, cls.weight, cls.bias, ptr.query.weight, ptr.query.bias, ptr.key.weight, ptr.key.bias, ocr_mask_add)
+            else:
+                s = Fn.M4CScoresFn.apply(x.view(B, W, H), mmt_ocr_output, cls.weight, cls.bias, ptr.query.weight, ptr.query.bias, ptr.key.weight, ptr.key.bias, ocr_mask_add,
+                                         Fn.shadows.get(cls.weight), Fn.shadows.get(ptr.query.weight), Fn.shadows.get(ptr.key.weight))
+            beams = decoding.select_beams(s.view(B * W, V + N), beams.scores, beams.finished, eos=eos, history=beams.history, step=i)
+            tokens = beams.tokens
+            seen.append(s)
+            parents.append(beams.parents)
+            if i + 1 < D:
+                cache.reorder(beams.parents)
+        # the score rows along the best beam, from the last step back
+        out = torch.empty(B, D, V + N, dtype=torch.float32, device=dev)
+        at = torch.zeros(B, dtype=torch.long, device=dev)
+        batch = torch.arange(B, device=dev)
+        for i in reversed(range(D)):
+            at = parents[i][batch, at]
+            out[:, i] = seen[i][batch, at]
+        fwd_results["scores"] = out
+        fwd_results["beam_tokens"], fwd_results["beam_scores"] = beams.history, beams.scores
+        prev = torch.zeros_like(sample_list["train_prev_inds"])
+        prev[:, 0] = int(self.answer_processor.BOS_IDX)
+        prev[:, 1:] = beams.history[:, 0, :D - 1]
         fwd_results["prev_inds"] = prev
         fwd_results["mmt_ocr_output"] = mmt_ocr_output
 
