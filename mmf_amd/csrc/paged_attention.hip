@@ -24,14 +24,15 @@ typedef const __attribute__((address_space(1))) void* glb_vp;
 static __device__ uint4 g_zero16;
 
 constexpr int STEP_ROWS = 32, CHUNK_ROWS = 128;
-constexpr int UNITS_MAX = 1024;        // requests (chunks) or groups of beams (steps) per launch
-constexpr int PREFIX_MAX = 3 * (UNITS_MAX + 1) * 4;
+constexpr int UNITS_MAX = 960;         // requests (chunks) or groups of beams (steps) per launch
+constexpr int PREFIX_MAX = 4 * (UNITS_MAX + 1) * 4;
 
 struct Args {
     mmf_paged_attn_desc d;
     int page_shift, group;             // group: query heads per key head
     int units, nb, per_group;          // nb: beams a unit takes together (steps), per_group: units per group of beams
     int target, run_min;               // workgroups to aim at when keys are split; shortest run
+    int parts;                         // partial results that the workspace has room for
     int split, tiles;                  // whether keys may be split at all; row tiles of the longest request
     float c;                           // |scale| log2 e (1 when scale is 0)
     uint32_t q_and, q_xor;             // the scale's sign on the queries' bits: their sign bits turned over (scale < 0), all bits cleared (scale 0)
@@ -41,32 +42,43 @@ struct Args {
 template <int RB> DEVI int swz(int row) { return RB == 128 ? (row >> 1) & 7 : ((row & 3) << 2) | ((row >> 2) & 3); }
 template <int RB> DEVI int at(int row, int chunk) { return row * RB + ((chunk ^ swz<RB>(row)) << 4); }
 
-// keys key0 .. + ROWS of one page run into K and V images by LDS-DMA; keys >= end, and keys on pages outside the pool, come as zeros.
-// `page` holds, in lane l, the page of key0 + (l % ROWS).  NW waves share the tile, this is wave `wave`.
-template <typename T, int D, int ROWS, int NW>
-DEVI void stage(const Args& a, int key0, int end, int page, int64_t head_off, unsigned char* k_img, unsigned char* v_img, int wave, int lane) {
-    constexpr int RB = D * (int)sizeof(T), CPR = RB / 16, RPI = 64 / CPR;
-    const int mask = a.d.page_size - 1;
+// Keys key0 .. + ROWS into K and V images by LDS-DMA; keys >= end, and keys on pages outside the pool, come as zeros.  `page` holds, in lane l, the page of
+// key0 + (l % ROWS).  NW waves share the tile.  What does not change from tile to tile is kept: a tile starts on a page, or ROWS divide the page and the
+// tile's start, so a key's place in its page is the tile's and the row's, added.
+template <typename T, int D, int ROWS, int NW> struct Stager {
+    static constexpr int RB = D * (int)sizeof(T), CPR = RB / 16, RPI = 64 / CPR, N = ROWS / (NW * RPI);
+    uint64_t k_row[N];                 // address of a row's 16 bytes in page 0
+    int64_t to_v;
+    uint32_t page_bytes;
+    DEVI Stager(const Args& a, int64_t head_off, int wave, int lane) {
+        page_bytes = (uint32_t)(a.d.page_stride * (int)sizeof(T));
+        to_v = (const char*)a.d.v_cache - (const char*)a.d.k_cache;
 #pragma unroll
-    for (int r0 = 0; r0 < ROWS; r0 += NW * RPI) {
-        const int row = r0 + wave * RPI + lane / CPR;
-        const int p = __shfl(page, row, 64);
-        const bool in = key0 + row < end, ok = in && (unsigned)p < (unsigned)a.d.pages;
-        if (in != ok) flag_page_error();
-        const int64_t off = (int64_t)p * a.d.page_stride + (int64_t)((key0 + row) & mask) * a.d.pos_stride + head_off;
-        const int byte = ((lane % CPR) ^ swz<RB>(row)) * 16;
-        const char* zero = reinterpret_cast<const char*>(&g_zero16);
-        const char* ks = ok ? (const char*)a.d.k_cache + off * (int)sizeof(T) + byte : zero;
-        const char* vs = ok ? (const char*)a.d.v_cache + off * (int)sizeof(T) + byte : zero;
-        const int to = (r0 + wave * RPI) * RB;
-        __builtin_amdgcn_global_load_lds((glb_vp)ks, (lds_vp)(k_img + to), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((glb_vp)vs, (lds_vp)(v_img + to), 16, 0, 0);
+        for (int i = 0; i < N; ++i) {
+            const int row = i * NW * RPI + wave * RPI + lane / CPR;
+            k_row[i] = (uint64_t)a.d.k_cache + (uint64_t)(head_off + (int64_t)(row & (a.d.page_size - 1)) * a.d.pos_stride) * sizeof(T) + ((lane % CPR) ^ swz<RB>(row)) * 16;
+        }
     }
-}
-// the page of key key0 + l % ROWS, for lane l; -1 behind the end
+    DEVI void operator()(const Args& a, int key0, int end, int page, unsigned char* k_img, unsigned char* v_img, int wave, int lane) const {
+        const bool in = key0 + (lane & (ROWS - 1)) < end, ok = in && (unsigned)page < (unsigned)a.d.pages;
+        if (in != ok) flag_page_error();
+        const int use = ok ? page : -1;
+        const uint64_t in_page = (uint64_t)((key0 & (a.d.page_size - 1)) * a.d.pos_stride) * sizeof(T);
+        const uint64_t zero = (uint64_t)&g_zero16;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int p = __shfl(use, i * NW * RPI + wave * RPI + lane / CPR, 64);
+            const uint64_t k = k_row[i] + (uint64_t)(uint32_t)p * page_bytes + in_page;
+            const uint64_t kk = p >= 0 ? k : zero, vv = p >= 0 ? k + to_v : zero;
+            const int to = (i * NW * RPI + wave * RPI) * RB;
+            __builtin_amdgcn_global_load_lds((glb_vp)kk, (lds_vp)(k_img + to), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((glb_vp)vv, (lds_vp)(v_img + to), 16, 0, 0);
+        }
+    }
+};
+// The page of key key0 + l % ROWS, for lane l (behind the end: any).  No branch: the value is first looked at a tile later, and may not be waited for before.
 template <int ROWS> DEVI int page_of(const Args& a, const int32_t* table, int key0, int end, int lane) {
-    const int key = key0 + (lane & (ROWS - 1));
-    return key < end ? table[key >> a.page_shift] : -1;
+    return table[max(min(key0 + (lane & (ROWS - 1)), end - 1), 0) >> a.page_shift];
 }
 
 DEVI void pick(f32x16& o, const f32x16& x, bool take) {
@@ -74,9 +86,51 @@ DEVI void pick(f32x16& o, const f32x16& x, bool take) {
     for (int r = 0; r < 16; ++r) o[r] = take ? x[r] : o[r];
 }
 
-// ---- the rows of a wave: their queries, softmax state and sums ----
+// ---- the rows of a wave: their queries, and the operands of a tile of NS x 32 keys as the two products take them ----
+// A tile's operands are all read before the first product that needs them: keys, then the score products; values, which land while the softmax is worked out, then
+// the products that add them up.  Left to itself the compiler reads each operand right before its product, and waits for LDS 32 times a tile.
+template <typename T, int D, int NS> struct Operands;
 template <typename T, int D> struct Rows;
 
+template <int D, int NS> struct Operands<bf16, D, NS> {
+    bf16x8 k[NS][D / 16], v[2 * NS][D / 32];
+    DEVI void read_k(const unsigned char* img, int lane) {
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) k[n][u] = *reinterpret_cast<const bf16x8*>(img + at<2 * D>(32 * n + (lane & 31), 2 * u + (lane >> 5)));
+    }
+    // V^T by ds_read_b64_tr_b16 (16 lanes read 4 rows x 16 columns, lane i gets column i): step u takes keys 16 u .. + 16 in the order that a lane holds their scores.
+    // Eight reads and their wait in one block: before a transposed read of its own the compiler waits for every load into LDS under way, the next tile's among them.
+    DEVI void read_v(const unsigned char* img, int lane) {
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        constexpr int T = D / 32, U = 4 / T;                       // column blocks of a step, steps of a block of reads
+        const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
+        const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)img;
+        uint32_t a[8];                                             // rows + 16: the same chunks of the swizzle, 16 rows on
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int col = 32 * (k / 2 % T) + 16 * (g & 1) + (i & 3) * 4;
+            a[k] = base + at<2 * D>(row + 8 * (k & 1), col >> 3) + (col & 7) * 2 + k / 2 / T * 32 * D;
+        }
+#pragma unroll
+        for (int b = 0; b < 2 * NS / U; ++b) {
+            s16x4 r[8];
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %8 offset:%c16\n\tds_read_b64_tr_b16 %1, %9 offset:%c16\n\tds_read_b64_tr_b16 %2, %10 offset:%c16\n\t"
+                "ds_read_b64_tr_b16 %3, %11 offset:%c16\n\tds_read_b64_tr_b16 %4, %12 offset:%c16\n\tds_read_b64_tr_b16 %5, %13 offset:%c16\n\t"
+                "ds_read_b64_tr_b16 %6, %14 offset:%c16\n\tds_read_b64_tr_b16 %7, %15 offset:%c16\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "i"(b * U * 32 * D)
+                : "memory");
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const s16x8 x = __builtin_shufflevector(r[2 * k], r[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                v[b * U + k / T][k % T] = __builtin_bit_cast(bf16x8, x);
+            }
+        }
+    }
+};
 template <int D> struct Rows<bf16, D> {
     bf16x8 q[D / 16];
     DEVI void load(const bf16* p, bool ok, const Args& a, int lane) {
@@ -87,42 +141,58 @@ template <int D> struct Rows<bf16, D> {
             q[s] = __builtin_bit_cast(bf16x8, (x & a.q_and) ^ (a.q_xor | a.q_xor >> 16));
         }
     }
-    // scores of keys row0 .. + 32 of the image
-    DEVI f32x16 scores(const unsigned char* k, int row0, int lane) const {
-        f32x16 s = {};
+    template <int NS> DEVI void scores(const Operands<bf16, D, NS>& x, f32x16 (&s)[NS]) const {
 #pragma unroll
         for (int u = 0; u < D / 16; ++u)
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(k + at<2 * D>(row0 + (lane & 31), 2 * u + (lane >> 5))), q[u], s, 0, 0, 0);
-        return s;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.k[n][u], q[u], s[n], 0, 0, 0);
     }
-    // sums += V^T p for keys row0 .. + 32 (PICK: in the lanes that `take`; a value that is no number stays with them); the transposed operand comes by ds_read_b64_tr_b16 (16 lanes read 4 rows x 16 columns, lane i gets column i)
-    template <bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16& p, const unsigned char* v, int row0, bool take, int lane) {
-        typedef s16x4 __attribute__((address_space(3))) * lds_p;
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const int g = lane >> 4, i = lane & 15;
-        bf16x8 pb[2];                                              // rounded to bf16: relative 2^-8 of each probability, the pool's own precision
+    // sums += V^T p (PICK: in the lanes that `take`; a value that is no number stays with them).  p is rounded to bf16: relative 2^-8 of each, the pool's own precision.
+    template <int NS, bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16 (&p)[NS], const Operands<bf16, D, NS>& x, bool take) {
+        bf16x8 pb[2 * NS];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pb[e >> 3][e & 7] = (bf16)p[e];
+        for (int u = 0; u < 2 * NS; ++u)
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t) {
-            f32x16 acc = o[t];
+            for (int e = 0; e < 8; ++e) pb[u][e] = (bf16)p[u >> 1][8 * (u & 1) + e];
+        if (PICK) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int row = row0 + 16 * u + 4 * (g >> 1) + (i >> 2), col = 32 * t + 16 * (g & 1) + (i & 3) * 4;
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(v + at<2 * D>(row, col >> 3) + (col & 7) * 2));
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(v + at<2 * D>(row + 8, col >> 3) + (col & 7) * 2));
-                const s16x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), pb[u], acc, 0, 0, 0);
+            for (int t = 0; t < D / 32; ++t) {
+                f32x16 acc = o[t];
+#pragma unroll
+                for (int u = 0; u < 2 * NS; ++u) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[u][t], pb[u], acc, 0, 0, 0);
+                pick(o[t], acc, take);
             }
-            if (PICK) pick(o[t], acc, take);
-            else o[t] = acc;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2 * NS; ++u)
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[u][t], pb[u], o[t], 0, 0, 0);
         }
     }
 };
 
 // fp32: a step of v_mfma_f32_32x32x2_f32 takes one element per lane, lanes 0 - 31 of reduction slot 0 and lanes 32 - 63 of slot 1
+template <int D, int NS> struct Operands<float, D, NS> {
+    f32x4 k[NS][D / 8];                                            // element (t, e) of half h: column 8 t + 4 h + e
+    float v[16 * NS][D / 32];                                      // step r of half h: key 8 (r / 4) + 4 h + r % 4, as a lane holds the scores
+    DEVI void read_k(const unsigned char* img, int lane) {
+#pragma unroll
+        for (int t = 0; t < D / 8; ++t)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) k[n][t] = *reinterpret_cast<const f32x4*>(img + at<4 * D>(32 * n + (lane & 31), 2 * t + (lane >> 5)));
+    }
+    DEVI void read_v(const unsigned char* img, int lane) {
+#pragma unroll
+        for (int r = 0; r < 16 * NS; ++r)
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) {
+                const int row = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), col = 32 * t + (lane & 31);
+                v[r][t] = *reinterpret_cast<const float*>(img + at<4 * D>(row, col >> 2) + (col & 3) * 4);
+            }
+    }
+};
 template <int D> struct Rows<float, D> {
-    f32x4 q[D / 8];                                                // element (t, e) of half h: column 8 t + 4 h + e
+    f32x4 q[D / 8];
     DEVI void load(const float* p, bool ok, const Args& a, int lane) {
 #pragma unroll
         for (int t = 0; t < D / 8; ++t) {
@@ -131,41 +201,65 @@ template <int D> struct Rows<float, D> {
             q[t] = __builtin_bit_cast(f32x4, (x & a.q_and) ^ a.q_xor);
         }
     }
-    DEVI f32x16 scores(const unsigned char* k, int row0, int lane) const {
-        f32x16 s = {};
+    template <int NS> DEVI void scores(const Operands<float, D, NS>& x, f32x16 (&s)[NS]) const {
 #pragma unroll
-        for (int t = 0; t < D / 8; ++t) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(k + at<4 * D>(row0 + (lane & 31), 2 * t + (lane >> 5)));
+        for (int t = 0; t < D / 8; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[t][e], s, 0, 0, 0);
-        }
-        return s;
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.k[n][t][e], q[t][e], s[n], 0, 0, 0);
     }
-    template <bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16& p, const unsigned char* v, int row0, bool take, int lane) {
+    template <int NS, bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16 (&p)[NS], const Operands<float, D, NS>& x, bool take) {
+        if (PICK) {
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t) {
-            f32x16 acc = o[t];
+            for (int t = 0; t < D / 32; ++t) {
+                f32x16 acc = o[t];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = row0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), col = 32 * t + (lane & 31);
-                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(v + at<4 * D>(row, col >> 2) + (col & 3) * 4), p[r], acc, 0, 0, 0);
+                for (int r = 0; r < 16 * NS; ++r) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[r][t], p[r >> 4][r & 15], acc, 0, 0, 0);
+                pick(o[t], acc, take);
             }
-            if (PICK) pick(o[t], acc, take);
-            else o[t] = acc;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16 * NS; ++r)
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[r][t], p[r >> 4][r & 15], o[t], 0, 0, 0);
         }
     }
 };
 
-DEVI float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// a value and that of lane ^ 32: v_permlane32_swap_b32 leaves the lower half's in one register and the upper half's in the other (the second copy is kept
+// apart from the first: of two equal operands the compiler returns the first result for both)
+DEVI void halves(float x, float& lower, float& upper) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    uint32_t v = u;
+    asm("" : "+v"(v));
+    const auto r = __builtin_amdgcn_permlane32_swap(u, v, false, false);
+    lower = __builtin_bit_cast(float, (uint32_t)r[0]);
+    upper = __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+DEVI float max_halves(float x) { float a, b; halves(x, a, b); return fmaxf(a, b); }
+DEVI float add_halves(float x) { float a, b; halves(x, a, b); return a + b; }
+DEVI int wave_min(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
 
 // One tile of NS x 32 keys, key0 its first, for the rows of a wave; lim: keys this lane's row sees.  m (in units of log2) may lag up to 8 behind the largest score:
 // a probability is then at most 2^8, and the sums need no rescaling on most tiles.
-template <typename T, int D, int NS, bool PICK = false>
+template <typename T, int D, int NS, bool PICK>
 DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsigned char* v, int key0, int lim, bool masked, float c, float& m, float& l, f32x16 (&o)[D / 32],
-                    int lane, bool take = true) {
-    f32x16 s[NS];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) s[n] = rows.scores(k, 32 * n, lane);
+                    int lane, bool take) {
+    f32x16 s[NS] = {};
+    Operands<T, D, NS> x;
+    x.read_k(k, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);                                           // a wave at its products goes before one at its softmax
+    rows.template scores<NS>(x, s);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+    x.read_v(v, lane);
+    __builtin_amdgcn_sched_barrier(0);
     float top = -INFINITY;
     const int h4 = 4 * (lane >> 5);
     if (masked) {
@@ -179,7 +273,7 @@ DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsign
     for (int n = 0; n < NS; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-    top = fmaxf(top, other_half(top)) * c;
+    top = max_halves(top) * c;
     if (__ballot(top > m + 8.f) != 0) {
         const float next = fmaxf(m, top), keep = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - next);
         m = next;
@@ -199,8 +293,9 @@ DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsign
             sum += s[n][r];
         }
     l += sum;
-#pragma unroll
-    for (int n = 0; n < NS; ++n) Rows<T, D>::template add<PICK>(o, s[n], v, 32 * n, take, lane);
+    __builtin_amdgcn_s_setprio(1);
+    Rows<T, D>::template add<NS, PICK>(o, s, x, take);
+    __builtin_amdgcn_s_setprio(0);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -223,7 +318,8 @@ DEVI Unit unit_of(const Args& a, int u) {
 
 struct Plan {
     int run, items, parts, joins;
-    int* item0;      // [units + 1] first item of each unit
+    int* order;      // [units] the units, longest first (up to 64 of them: else as they come)
+    int* item0;      // [units + 1] first item of each unit, in that order
     int* part0;      // first partial result (units with several runs)
     int* join0;      // first (tile, head) to join
 };
@@ -249,7 +345,7 @@ DEVI int wave_sum_int(int v) {
     return v;
 }
 
-// `lds`: 3 (units + 1) ints; every wave ends with the same plan (the first one writes it).  Where nothing can be split (all lengths within the shortest run) there is
+// `lds`: 4 (units + 1) ints; every wave ends with the same plan (the first one writes it).  Where nothing can be split (all lengths within the shortest run) there is
 // nothing to plan: item = (unit, tile of the longest request, head).
 template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     const int lane = threadIdx.x & 63;
@@ -262,6 +358,7 @@ template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     p.item0 = lds;
     p.part0 = lds + a.units + 1;
     p.join0 = lds + 2 * (a.units + 1);
+    p.order = lds + 3 * (a.units + 1);
     int64_t work = 0;
     for (int u = lane; u < a.units; u += 64) {
         const Unit x = unit_of(a, u);
@@ -269,28 +366,44 @@ template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     }
     work = wave_add(work) * a.d.kv_heads;
     int64_t want = (work + a.target - 1) / a.target;
-    // steps: each request's last run is a short one; lengthen the runs until the workgroups that are resident together hold all of them
+    // Steps: each request's last run is a short one; lengthen the runs until the workgroups that are resident together hold all of them.
+    // Either: lengthen them until the partial results have room.
 #pragma unroll 1
-    for (int round = 0; round < (TILE == STEP_ROWS ? 4 : 1); ++round) {
-        p.run = (int)((max((int64_t)a.run_min, min(want, (int64_t)0x1fffffff)) + 63) / 64 * 64);
-        int n = 0, runs_most = 0;
+    for (int round = 0;; ++round) {
+        p.run = round < 12 ? (int)((max((int64_t)a.run_min, min(want, (int64_t)0x1fffffff)) + 63) / 64 * 64) : 0x3fffffff;
+        int n = 0, split = 0;
         for (int u = lane; u < a.units; u += 64) {
             const Unit x = unit_of(a, u);
-            const int runs = max(1, (x.kv + p.run - 1) / p.run);
-            n += tiles_of<TILE>(a, x) * a.d.kv_heads * runs;
-            runs_most = max(runs_most, runs);
+            const int runs = max(1, (int)(((int64_t)x.kv + p.run - 1) / p.run)), k = tiles_of<TILE>(a, x) * a.d.kv_heads * runs;
+            n += k;
+            if (runs > 1) split += k;
         }
         n = wave_sum_int(n);
-        if (n <= a.target || __ballot(runs_most > 1) == 0) break;
-        want = (int64_t)p.run * n / a.target + 1;
+        split = wave_sum_int(split);
+        if (split <= a.parts && (TILE != STEP_ROWS || split == 0 || n <= a.target || round >= 4)) break;
+        want = (int64_t)p.run + (int64_t)p.run * max(n - a.target, a.target / 8) / a.target;
     }
+    // longest first: workgroups that come free late then get short work (makespan over 6 requests of 1711 .. 16771 keys: 1.07 of the mean, 1.4 in any order)
+    if (a.units <= 64) {
+        const int mine = lane < a.units ? unit_of(a, lane).kv : -1;
+        int rank = 0;
+#pragma unroll 4
+        for (int v = 0; v < a.units; ++v) {
+            const int kv = __builtin_amdgcn_readlane(mine, v);
+            rank += kv > mine || (kv == mine && v < lane);
+        }
+        if (lane < a.units) p.order[rank] = lane;
+    } else {
+        for (int u = lane; u < a.units; u += 64) p.order[u] = u;
+    }
+    __syncthreads();
     int items = 0, parts = 0, joins = 0;
     for (int u0 = 0; u0 < a.units; u0 += 64) {
         const int u = u0 + lane;
         int i = 0, q = 0, j = 0;
         if (u < a.units) {
-            const Unit x = unit_of(a, u);
-            const int t = tiles_of<TILE>(a, x) * a.d.kv_heads, runs = max(1, (x.kv + p.run - 1) / p.run);
+            const Unit x = unit_of(a, p.order[u]);
+            const int t = tiles_of<TILE>(a, x) * a.d.kv_heads, runs = max(1, (int)(((int64_t)x.kv + p.run - 1) / p.run));
             i = t * runs;
             if (runs > 1) { q = i; j = t; }
         }
@@ -317,13 +430,13 @@ DEVI int find(const int* first, int units, int i) {          // the last unit wh
     return lo;
 }
 
-// unit, run, tile and head of an item
+// place in the order, run, tile and head of an item
 struct Item { int u, run, tile, head; Unit x; };
 template <int TILE> DEVI Item item_of(const Args& a, const Plan& plan, int item) {
     Item it;
     if (a.split) {
         it.u = find(plan.item0, a.units, item);
-        it.x = unit_of(a, it.u);
+        it.x = unit_of(a, plan.order[it.u]);
         int rest = item - plan.item0[it.u];
         it.head = rest % a.d.kv_heads;
         rest /= a.d.kv_heads;
@@ -363,7 +476,7 @@ template <typename T, int D> DEVI T* out_row(const Args& a, const Row& r, int h)
 }
 // partial results: [part][TILE][D] sums, then [part][TILE][2] maximum (log2) and sum
 template <int D, int TILE> DEVI float* part_o(const Args& a, int part) { return (float*)a.d.ws + (int64_t)part * TILE * D; }
-template <int D, int TILE> DEVI float* part_ml(const Args& a, int part) { return (float*)a.d.ws + (int64_t)2 * a.target * TILE * D + (int64_t)part * TILE * 2; }
+template <int D, int TILE> DEVI float* part_ml(const Args& a, int part) { return (float*)a.d.ws + (int64_t)a.parts * TILE * D + (int64_t)part * TILE * 2; }
 
 DEVI void store4(bf16* p, float a, float b, float c, float d) { *reinterpret_cast<bf16x4*>(p) = pack4(a, b, c, d); }
 DEVI void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d}; }
@@ -393,17 +506,17 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         const int lim = row.token >= 0 ? sees(a, x, row.i) : 0x7fffffff;      // (rows without a token compute on zeros: nothing of them is written)
         Rows<T, D> rows;
         rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a, lane);
-        int free_to = lim;                                                       // keys every row of the wave sees
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) free_to = min(free_to, __shfl_xor(free_to, o, 64));
+        const int free_to = wave_min(lim), see_to = -wave_min(row.token >= 0 ? -lim : 0);       // keys that every row of the wave sees, that any does
+        const bool idle = row0 + 32 * wave >= x.n * a.group;                     // a wave without rows only helps to stage
         float m = -INFINITY, l = 0.f;
         f32x16 o[D / 32] = {};
         const int32_t* table = a.d.tables + x.req * a.d.table_row;
         const int64_t head_off = h * a.d.head_stride;
         const int steps = end > start ? (end - start + KT - 1) / KT : 0;
+        const Stager<T, D, KT, 4> stage(a, head_off, wave, lane);
         int page = page_of<KT>(a, table, start, end, lane);
         __syncthreads();                                                         // the item before has read its last tile
-        if (steps > 0) stage<T, D, KT, 4>(a, start, end, page, head_off, lds, lds + IMG, wave, lane);
+        if (steps > 0) stage(a, start, end, page, lds, lds + IMG, wave, lane);
         page = page_of<KT>(a, table, start + KT, end, lane);
         for (int j = 0; j < steps; ++j) {
             const int key0 = start + j * KT;
@@ -412,12 +525,17 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
             __syncthreads();
             if (j + 1 < steps) {
                 unsigned char* next = lds + ((j + 1) & 1) * 2 * IMG;
-                stage<T, D, KT, 4>(a, key0 + KT, end, page, head_off, next, next + IMG, wave, lane);
+                stage(a, key0 + KT, end, page, next, next + IMG, wave, lane);
                 page = page_of<KT>(a, table, key0 + 2 * KT, end, lane);
             }
-            tile_step<T, D, NS>(rows, img, img + IMG, key0, min(lim, end), key0 + KT > min(free_to, end), a.c, m, l, o, lane);
+            // 32 keys at a time: the operands of 64 together with the sums would not fit the registers of two waves on a SIMD
+            const int subs = idle ? 0 : (min(min(see_to, end) - key0, KT) + 31) >> 5;
+#pragma unroll 1
+            for (int n = 0; n < subs; ++n)
+                tile_step<T, D, 1, false>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane,
+                                          true);
         }
-        l += other_half(l);
+        l = add_halves(l);
         if (whole) {
             if (row.token >= 0) {
                 T* out = out_row<T, D>(a, row, h);
@@ -471,9 +589,7 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         const int lim = row.token >= 0 ? sees(a, x, row.i) : 0x7fffffff;
         Rows<T, D> rows;
         rows.load((const T*)a.d.q + row.token * a.d.q_row + (int64_t)(h * a.group + row.head) * a.d.q_head, row.token >= 0, a, lane);
-        int free_to = lim;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) free_to = min(free_to, __shfl_xor(free_to, o, 64));
+        const int free_to = wave_min(lim);
         const int32_t* table = a.d.tables + x.req * a.d.table_row;
         const int64_t head_off = h * a.d.head_stride;
         // pages that are the same for every beam are read once for all of them: up to the first block that differs
@@ -508,8 +624,9 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         f32x16 o[D / 32] = {};
         Job now = job(wave), next = job(wave + 4);
         int page_now = pages(now), page_next = pages(next);
+        const Stager<T, D, 32, 1> stage(a, head_off, 0, lane);
         constexpr int LOADS = 2 * 32 * RB / 1024;                                // LDS-DMA instructions of a tile
-        if (BUF == 2 && wave < jobs) stage<T, D, 32, 1>(a, now.key0, now.end, page_now, head_off, mine, mine + IMG, 0, lane);
+        if (BUF == 2 && wave < jobs) stage(a, now.key0, now.end, page_now, mine, mine + IMG, 0, lane);
         for (int j = wave; j < jobs; j += 4) {
             unsigned char* img = mine + (BUF == 2 ? ((j >> 2) & 1) * 2 * IMG : 0);
             const Job after = job(j + 8);
@@ -517,13 +634,13 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
             if (BUF == 2) {
                 if (j + 4 < jobs) {
                     unsigned char* to = mine + (((j >> 2) + 1) & 1) * 2 * IMG;
-                    stage<T, D, 32, 1>(a, next.key0, next.end, page_next, head_off, to, to + IMG, 0, lane);
+                    stage(a, next.key0, next.end, page_next, to, to + IMG, 0, lane);
                     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");  // this tile's loads are older than the last LOADS
                 } else {
                     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 }
             } else {
-                stage<T, D, 32, 1>(a, now.key0, now.end, page_now, head_off, img, img + IMG, 0, lane);
+                stage(a, now.key0, now.end, page_now, img, img + IMG, 0, lane);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
             const int see = min(lim, now.end);
@@ -533,7 +650,7 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
             now = next; next = after;
             page_now = page_next; page_next = page_after;
         }
-        l += other_half(l);
+        l = add_halves(l);
         // the four waves' sums meet: [wave][row][D] fp32 in the tiles' place, [wave][row][2] behind
         __syncthreads();
         constexpr int LD = D + 4;                                                // (rows of D floats alone would put every row's column on one bank)
@@ -592,7 +709,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(Args a) {
     for (int i = blockIdx.x; i < plan.joins * SLICES; i += gridDim.x) {
         const int j = i / SLICES, slice = i - j * SLICES;
         const int u = find(plan.join0, a.units, j);
-        const Unit x = unit_of(a, u);
+        const Unit x = unit_of(a, plan.order[u]);
         const int h = (j - plan.join0[u]) % a.d.kv_heads, tile = (j - plan.join0[u]) / a.d.kv_heads, tiles = tiles_of<TILE>(a, x);
         const int runs = (x.kv + plan.run - 1) / plan.run;
         const int at_row = slice * ROWS + threadIdx.x / PER, e = (threadIdx.x % PER) * 4;
@@ -627,16 +744,17 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(Args a) {
     }
 }
 
-struct Shape { bool chunk, split; int nb, target, run_min; int64_t ws; };
+struct Shape { bool chunk, split; int nb, target, run_min, parts; int64_t ws; };
 Shape shape_of(const mmf_paged_attn_desc* d) {
     Shape s;
     const int64_t rows = (int64_t)d->max_q * (d->heads / d->kv_heads);
     s.chunk = rows > STEP_ROWS;
     s.nb = s.chunk ? 1 : (int)(STEP_ROWS / rows < d->beams ? STEP_ROWS / rows : d->beams);
-    s.target = s.chunk ? 1024 : 512;
+    s.target = s.chunk ? 768 : 512;
     s.run_min = s.chunk ? 1024 : 256;
+    s.parts = s.chunk ? 1536 : 1024;
     s.split = (int64_t)d->blocks * d->page_size > s.run_min;
-    s.ws = s.split ? (int64_t)2 * s.target * (s.chunk ? CHUNK_ROWS : STEP_ROWS) * (d->head_dim + 2) * 4 : 0;
+    s.ws = s.split ? (int64_t)s.parts * (s.chunk ? CHUNK_ROWS : STEP_ROWS) * (d->head_dim + 2) * 4 : 0;
     return s;
 }
 
@@ -659,6 +777,7 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
     a.nb = s.nb;
     a.per_group = (d->beams + s.nb - 1) / s.nb;
     a.target = s.target;
+    a.parts = s.parts;
     a.run_min = s.run_min;
     a.split = s.split;
     a.tiles = s.chunk ? (int)(((int64_t)d->max_q * a.group + CHUNK_ROWS - 1) / CHUNK_ROWS) : 1;
@@ -674,10 +793,10 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
         a.d.q_lens = d->q_lens + r0 / d->beams;
         a.d.q_start = d->q_start + r0;
         a.units = s.nb == 1 ? n : n / d->beams * a.per_group;
-        const int prefix = 3 * (a.units + 1) * 4;
+        const int prefix = 4 * (a.units + 1) * 4;
         const int64_t most = (int64_t)a.tiles * a.units * d->kv_heads;
         MMF_CHECK_ARG(most <= 0x3fffffff, "paged_attention: too many rows for one call");
-        const int grid = s.split || most > s.target ? s.target : (int)most;
+        const int cap = s.chunk ? 2048 : 512, grid = s.split || most > cap ? cap : (int)most;
         if (s.chunk) {
             const int lds = chunk_lds<T, D> + prefix;
             static std::atomic<uint64_t> done{0};
@@ -728,6 +847,9 @@ int mmf_paged_attention(const mmf_paged_attn_desc* d, void* stream) {
     MMF_CHECK_ARG(((uintptr_t)d->q & 15) == 0 && ((uintptr_t)d->k_cache & 15) == 0 && ((uintptr_t)d->v_cache & 15) == 0 && ((uintptr_t)d->out & 15) == 0 &&
                       d->q_row % unit == 0 && d->q_head % unit == 0 && d->page_stride % unit == 0 && d->head_stride % unit == 0 && d->pos_stride % unit == 0 &&
                       d->out_row % unit == 0 && d->out_head % unit == 0, "paged_attention: rows start on 16 bytes");
+    const int64_t size = d->is_f32 ? 4 : 2;
+    MMF_CHECK_ARG(d->page_stride >= 0 && d->page_stride * size <= 0xffffffffll && d->pos_stride >= 0 && d->pos_stride * d->page_size * size <= 0x7fffffff && d->head_stride >= 0,
+                  "paged_attention: a page within 2 GiB, pages within 4 GiB of each other");
     if (d->tokens == 0) return 0;
     const Shape s = shape_of(d);
     MMF_CHECK_ARG(s.ws == 0 || (d->ws && ((uintptr_t)d->ws & 15) == 0), "paged_attention: null workspace");
