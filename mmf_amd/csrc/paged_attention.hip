@@ -47,28 +47,30 @@ template <int RB> DEVI int at(int row, int chunk) { return row * RB + ((chunk ^ 
 // tile's start, so a key's place in its page is the tile's and the row's, added.
 template <typename T, int D, int ROWS, int NW> struct Stager {
     static constexpr int RB = D * (int)sizeof(T), CPR = RB / 16, RPI = 64 / CPR, N = ROWS / (NW * RPI);
-    uint64_t k_row[N];                 // address of a row's 16 bytes in page 0
+    uint32_t in_page[N];               // a row's 16 bytes in its page
+    uint64_t head;                     // page 0 of the head
     int64_t to_v;
     uint32_t page_bytes;
     DEVI Stager(const Args& a, int64_t head_off, int wave, int lane) {
         page_bytes = (uint32_t)(a.d.page_stride * (int)sizeof(T));
         to_v = (const char*)a.d.v_cache - (const char*)a.d.k_cache;
+        head = (uint64_t)a.d.k_cache + (uint64_t)head_off * sizeof(T);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int row = i * NW * RPI + wave * RPI + lane / CPR;
-            k_row[i] = (uint64_t)a.d.k_cache + (uint64_t)(head_off + (int64_t)(row & (a.d.page_size - 1)) * a.d.pos_stride) * sizeof(T) + ((lane % CPR) ^ swz<RB>(row)) * 16;
+            in_page[i] = (uint32_t)((row & (a.d.page_size - 1)) * (uint32_t)a.d.pos_stride * sizeof(T)) + ((lane % CPR) ^ swz<RB>(row)) * 16;
         }
     }
     DEVI void operator()(const Args& a, int key0, int end, int page, unsigned char* k_img, unsigned char* v_img, int wave, int lane) const {
         const bool in = key0 + (lane & (ROWS - 1)) < end, ok = in && (unsigned)page < (unsigned)a.d.pages;
         if (in != ok) flag_page_error();
         const int use = ok ? page : -1;
-        const uint64_t in_page = (uint64_t)((key0 & (a.d.page_size - 1)) * a.d.pos_stride) * sizeof(T);
+        const uint64_t tile = head + (uint32_t)((key0 & (a.d.page_size - 1)) * (uint32_t)a.d.pos_stride * sizeof(T));
         const uint64_t zero = (uint64_t)&g_zero16;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int p = __shfl(use, i * NW * RPI + wave * RPI + lane / CPR, 64);
-            const uint64_t k = k_row[i] + (uint64_t)(uint32_t)p * page_bytes + in_page;
+            const uint64_t k = (uint64_t)(uint32_t)p * page_bytes + tile + in_page[i];
             const uint64_t kk = p >= 0 ? k : zero, vv = p >= 0 ? k + to_v : zero;
             const int to = (i * NW * RPI + wave * RPI) * RB;
             __builtin_amdgcn_global_load_lds((glb_vp)kk, (lds_vp)(k_img + to), 16, 0, 0);
@@ -101,34 +103,20 @@ template <int D, int NS> struct Operands<bf16, D, NS> {
             for (int n = 0; n < NS; ++n) k[n][u] = *reinterpret_cast<const bf16x8*>(img + at<2 * D>(32 * n + (lane & 31), 2 * u + (lane >> 5)));
     }
     // V^T by ds_read_b64_tr_b16 (16 lanes read 4 rows x 16 columns, lane i gets column i): step u takes keys 16 u .. + 16 in the order that a lane holds their scores.
-    // Eight reads and their wait in one block: before a transposed read of its own the compiler waits for every load into LDS under way, the next tile's among them.
     DEVI void read_v(const unsigned char* img, int lane) {
+        typedef s16x4 __attribute__((address_space(3))) * lds_p;
         typedef short s16x8 __attribute__((ext_vector_type(8)));
-        constexpr int T = D / 32, U = 4 / T;                       // column blocks of a step, steps of a block of reads
-        const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2);
-        const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)img;
-        uint32_t a[8];                                             // rows + 16: the same chunks of the swizzle, 16 rows on
+        const int g = lane >> 4, i = lane & 15;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int col = 32 * (k / 2 % T) + 16 * (g & 1) + (i & 3) * 4;
-            a[k] = base + at<2 * D>(row + 8 * (k & 1), col >> 3) + (col & 7) * 2 + k / 2 / T * 32 * D;
-        }
+        for (int u = 0; u < 2 * NS; ++u)
 #pragma unroll
-        for (int b = 0; b < 2 * NS / U; ++b) {
-            s16x4 r[8];
-            asm volatile(
-                "ds_read_b64_tr_b16 %0, %8 offset:%c16\n\tds_read_b64_tr_b16 %1, %9 offset:%c16\n\tds_read_b64_tr_b16 %2, %10 offset:%c16\n\t"
-                "ds_read_b64_tr_b16 %3, %11 offset:%c16\n\tds_read_b64_tr_b16 %4, %12 offset:%c16\n\tds_read_b64_tr_b16 %5, %13 offset:%c16\n\t"
-                "ds_read_b64_tr_b16 %6, %14 offset:%c16\n\tds_read_b64_tr_b16 %7, %15 offset:%c16\n\ts_waitcnt lgkmcnt(0)"
-                : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-                : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "i"(b * U * 32 * D)
-                : "memory");
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const s16x8 x = __builtin_shufflevector(r[2 * k], r[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-                v[b * U + k / T][k % T] = __builtin_bit_cast(bf16x8, x);
+            for (int t = 0; t < D / 32; ++t) {
+                const int row = 16 * u + 4 * (g >> 1) + (i >> 2), col = 32 * t + 16 * (g & 1) + (i & 3) * 4;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(img + at<2 * D>(row, col >> 3) + (col & 7) * 2));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(img + at<2 * D>(row + 8, col >> 3) + (col & 7) * 2));
+                const s16x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                v[u][t] = __builtin_bit_cast(bf16x8, x);
             }
-        }
     }
 };
 template <int D> struct Rows<bf16, D> {
@@ -245,11 +233,12 @@ DEVI int wave_min(int v) {
     return __builtin_amdgcn_readfirstlane(v);
 }
 
+// `ahead` is called once the tile's operands are read: loads into LDS that are under way when the transposed values are read would be waited for first.
 // One tile of NS x 32 keys, key0 its first, for the rows of a wave; lim: keys this lane's row sees.  m (in units of log2) may lag up to 8 behind the largest score:
 // a probability is then at most 2^8, and the sums need no rescaling on most tiles.
-template <typename T, int D, int NS, bool PICK>
+template <typename T, int D, int NS, bool PICK, typename F>
 DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsigned char* v, int key0, int lim, bool masked, float c, float& m, float& l, f32x16 (&o)[D / 32],
-                    int lane, bool take) {
+                    int lane, bool take, F ahead) {
     f32x16 s[NS] = {};
     Operands<T, D, NS> x;
     x.read_k(k, lane);
@@ -259,6 +248,8 @@ DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsign
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
     x.read_v(v, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    ahead();
     __builtin_amdgcn_sched_barrier(0);
     float top = -INFINITY;
     const int h4 = 4 * (lane >> 5);
@@ -450,6 +441,10 @@ template <int TILE> DEVI Item item_of(const Args& a, const Plan& plan, int item)
         it.run = 0;
         it.x = unit_of(a, it.u);
     }
+    // the same for the whole workgroup: in scalar registers from here on
+    int* f[] = {&it.u, &it.run, &it.tile, &it.head, &it.x.req, &it.x.nb, &it.x.n, &it.x.n_all, &it.x.kv};
+#pragma unroll
+    for (int k = 0; k < 9; ++k) *f[k] = __builtin_amdgcn_readfirstlane(*f[k]);
     if (it.tile == 0 && it.run == 0 && it.head == 0 && threadIdx.x == 0 && (it.x.n_all > a.d.max_q || it.x.kv != a.d.kv_lens[it.x.req / a.d.beams])) flag_page_error();
     return it;
 }
@@ -523,17 +518,17 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
             unsigned char* img = lds + (j & 1) * 2 * IMG;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (j + 1 < steps) {
-                unsigned char* next = lds + ((j + 1) & 1) * 2 * IMG;
-                stage(a, key0 + KT, end, page, next, next + IMG, wave, lane);
-                page = page_of<KT>(a, table, key0 + 2 * KT, end, lane);
-            }
-            // 32 keys at a time: the operands of 64 together with the sums would not fit the registers of two waves on a SIMD
+            auto ahead = [&] {
+                if (j + 1 < steps) {
+                    unsigned char* next = lds + ((j + 1) & 1) * 2 * IMG;
+                    stage(a, key0 + KT, end, page, next, next + IMG, wave, lane);
+                    page = page_of<KT>(a, table, key0 + 2 * KT, end, lane);
+                }
+            };
             const int subs = idle ? 0 : (min(min(see_to, end) - key0, KT) + 31) >> 5;
-#pragma unroll 1
-            for (int n = 0; n < subs; ++n)
-                tile_step<T, D, 1, false>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane,
-                                          true);
+            if (subs <= 0) { ahead(); continue; }
+            { const int n = 0; tile_step<T, D, 1, false>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane, true, ahead); }
+            if (subs == 2) { const int n = 1; tile_step<T, D, 1, false>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane, true, [] {}); }
         }
         l = add_halves(l);
         if (whole) {
@@ -566,16 +561,15 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
 // ------------------------------------------------------------------------------------------------
 // steps
 // ------------------------------------------------------------------------------------------------
-template <typename T, int D> constexpr int step_buffers = D * (int)sizeof(T) <= 128 ? 2 : 1;
-template <typename T, int D> constexpr int step_lds = step_buffers<T, D> * 4 * 2 * 32 * D * (int)sizeof(T);       // one or two tiles of 32 keys per wave
+template <typename T, int D> constexpr int step_lds = 4 * 2 * 32 * D * (int)sizeof(T);       // a tile of 32 keys per wave
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_attn_step_kernel(Args a) {
     extern __shared__ unsigned char lds[];
-    constexpr int RB = D * (int)sizeof(T), IMG = 32 * RB, BUF = step_buffers<T, D>;
+    constexpr int RB = D * (int)sizeof(T), IMG = 32 * RB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned char* mine = lds + wave * BUF * 2 * IMG;
-    int* shared_to = reinterpret_cast<int*>(lds + BUF * 8 * IMG);
+    unsigned char* mine = lds + wave * 2 * IMG;
+    int* shared_to = reinterpret_cast<int*>(lds + 8 * IMG);
     const Plan plan = make_plan<STEP_ROWS>(a, shared_to + 4);
     for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
         const Item it = item_of<STEP_ROWS>(a, plan, item);
@@ -623,32 +617,22 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         float m = -INFINITY, l = 0.f;
         f32x16 o[D / 32] = {};
         Job now = job(wave), next = job(wave + 4);
-        int page_now = pages(now), page_next = pages(next);
+        int page = pages(now), page_next = pages(next);
         const Stager<T, D, 32, 1> stage(a, head_off, 0, lane);
-        constexpr int LOADS = 2 * 32 * RB / 1024;                                // LDS-DMA instructions of a tile
-        if (BUF == 2 && wave < jobs) stage(a, now.key0, now.end, page_now, mine, mine + IMG, 0, lane);
+        if (wave < jobs) stage(a, now.key0, now.end, page, mine, mine + IMG, 0, lane);
         for (int j = wave; j < jobs; j += 4) {
-            unsigned char* img = mine + (BUF == 2 ? ((j >> 2) & 1) * 2 * IMG : 0);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             const Job after = job(j + 8);
-            const int page_after = pages(after);                                 // (older than the loads of the next tile: waiting for it leaves those in flight)
-            if (BUF == 2) {
-                if (j + 4 < jobs) {
-                    unsigned char* to = mine + (((j >> 2) + 1) & 1) * 2 * IMG;
-                    stage(a, next.key0, next.end, page_next, to, to + IMG, 0, lane);
-                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");  // this tile's loads are older than the last LOADS
-                } else {
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                }
-            } else {
-                stage(a, now.key0, now.end, page_now, img, img + IMG, 0, lane);
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
+            // once the tile's operands are in registers, the next tile lands in its place
+            auto ahead = [&] {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (j + 4 < jobs) stage(a, next.key0, next.end, page_next, mine, mine + IMG, 0, lane);
+                page_next = pages(after);
+            };
             const int see = min(lim, now.end);
             const bool take = now.beam < 0 || row.beam == now.beam;              // a tile of one beam: the other beams' rows see none of it
-            tile_step<T, D, 1, true>(rows, img, img + IMG, now.key0, take ? see : 0, now.beam >= 0 || now.key0 + 32 > min(free_to, now.end), a.c, m, l, o, lane, take);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                   // the tile is read before the next one lands on it
+            tile_step<T, D, 1, true>(rows, mine, mine + IMG, now.key0, take ? see : 0, now.beam >= 0 || now.key0 + 32 > min(free_to, now.end), a.c, m, l, o, lane, take, ahead);
             now = next; next = after;
-            page_now = page_next; page_next = page_after;
         }
         l = add_halves(l);
         // the four waves' sums meet: [wave][row][D] fp32 in the tiles' place, [wave][row][2] behind
