@@ -33,7 +33,7 @@ struct Args {
     int units, nb, per_group;          // nb: beams a unit takes together (steps), per_group: units per group of beams
     int target, run_min;               // workgroups to aim at when keys are split; shortest run
     int parts;                         // partial results that the workspace has room for
-    int split, tiles;                  // whether keys may be split at all; row tiles of the longest request
+    int split;                         // whether keys may be split at all
     float c;                           // |scale| log2 e (1 when scale is 0)
     uint32_t q_and, q_xor;             // the scale's sign on the queries' bits: their sign bits turned over (scale < 0), all bits cleared (scale 0)
 };
@@ -337,13 +337,13 @@ DEVI int wave_sum_int(int v) {
 }
 
 // `lds`: 4 (units + 1) ints; every wave ends with the same plan (the first one writes it).  Where nothing can be split (all lengths within the shortest run) there is
-// nothing to plan: item = (unit, tile of the longest request, head).
+// no run to choose, and steps have nothing to plan: item = (unit, head).
 template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     const int lane = threadIdx.x & 63;
     Plan p;
-    if (!a.split) {
-        p.run = 0x3fffffff;
-        p.items = a.units * a.tiles * a.d.kv_heads;
+    p.run = 0x3fffffff;
+    if (!a.split && TILE == STEP_ROWS) {
+        p.items = a.units * a.d.kv_heads;
         return p;
     }
     p.item0 = lds;
@@ -351,7 +351,7 @@ template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     p.join0 = lds + 2 * (a.units + 1);
     p.order = lds + 3 * (a.units + 1);
     int64_t work = 0;
-    for (int u = lane; u < a.units; u += 64) {
+    for (int u = a.split ? lane : a.units; u < a.units; u += 64) {
         const Unit x = unit_of(a, u);
         work += (int64_t)tiles_of<TILE>(a, x) * x.kv;
     }
@@ -360,7 +360,7 @@ template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     // Steps: each request's last run is a short one; lengthen the runs until the workgroups that are resident together hold all of them.
     // Either: lengthen them until the partial results have room.
 #pragma unroll 1
-    for (int round = 0;; ++round) {
+    for (int round = 0; a.split; ++round) {
         p.run = round < 12 ? (int)((max((int64_t)a.run_min, min(want, (int64_t)0x1fffffff)) + 63) / 64 * 64) : 0x3fffffff;
         int n = 0, split = 0;
         for (int u = lane; u < a.units; u += 64) {
@@ -425,7 +425,7 @@ DEVI int find(const int* first, int units, int i) {          // the last unit wh
 struct Item { int u, run, tile, head; Unit x; };
 template <int TILE> DEVI Item item_of(const Args& a, const Plan& plan, int item) {
     Item it;
-    if (a.split) {
+    if (a.split || TILE != STEP_ROWS) {
         it.u = find(plan.item0, a.units, item);
         it.x = unit_of(a, plan.order[it.u]);
         int rest = item - plan.item0[it.u];
@@ -435,10 +435,9 @@ template <int TILE> DEVI Item item_of(const Args& a, const Plan& plan, int item)
         it.tile = rest % tiles;
         it.run = rest / tiles;
     } else {
-        it.head = item % a.d.kv_heads;
-        it.tile = item / a.d.kv_heads % a.tiles;
-        it.u = item / a.d.kv_heads / a.tiles;
-        it.run = 0;
+        it.u = item / a.d.kv_heads;
+        it.head = item - it.u * a.d.kv_heads;
+        it.tile = it.run = 0;
         it.x = unit_of(a, it.u);
     }
     // the same for the whole workgroup: in scalar registers from here on
@@ -492,7 +491,6 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         const Item it = item_of<CHUNK_ROWS>(a, plan, item);
         const Unit& x = it.x;
         const int u = it.u, h = it.head, run = it.run, row0 = it.tile * CHUNK_ROWS;
-        if (row0 >= x.n * a.group) continue;                                     // (a tile that only the longest request has)
         const bool whole = plan.run >= x.kv;
         const int last = min(x.n * a.group, row0 + CHUNK_ROWS) - 1;
         const int end = min(sees(a, x, last / a.group), (run + 1) * plan.run);
@@ -764,7 +762,7 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
     a.parts = s.parts;
     a.run_min = s.run_min;
     a.split = s.split;
-    a.tiles = s.chunk ? (int)(((int64_t)d->max_q * a.group + CHUNK_ROWS - 1) / CHUNK_ROWS) : 1;
+    const int64_t tiles = s.chunk ? ((int64_t)d->max_q * a.group + CHUNK_ROWS - 1) / CHUNK_ROWS : 1;
     a.c = d->scale != 0.f ? fabsf(d->scale) * 1.44269504088896340736f : 1.f;
     a.q_and = d->scale != 0.f ? 0xffffffffu : 0u;
     a.q_xor = d->scale < 0.f ? 0x80000000u : 0u;
@@ -778,7 +776,7 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
         a.d.q_start = d->q_start + r0;
         a.units = s.nb == 1 ? n : n / d->beams * a.per_group;
         const int prefix = 4 * (a.units + 1) * 4;
-        const int64_t most = (int64_t)a.tiles * a.units * d->kv_heads;
+        const int64_t most = tiles * a.units * d->kv_heads;
         MMF_CHECK_ARG(most <= 0x3fffffff, "paged_attention: too many rows for one call");
         const int cap = s.chunk ? 2048 : 512, grid = s.split || most > cap ? cap : (int)most;
         if (s.chunk) {
