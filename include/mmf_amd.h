@@ -810,11 +810,11 @@ typedef struct mmf_beam_select_desc {
     const void* logits; int64_t ld;
     const float* scores; const uint8_t* finished; const int64_t* history;
     float* scores_out; int64_t* parents; int64_t* tokens; uint8_t* finished_out; int64_t* history_out;
-    void* ws;                                    /* mmf_beam_select_ws_bytes(groups, beams, vocab) bytes, 16-byte aligned */
+    void* ws;                                    /* mmf_beam_select_ws_bytes(groups, beams, vocab, is_f32) bytes, 16-byte aligned */
     int64_t vocab, eos, length, step;
     int groups, beams, is_f32;
 } mmf_beam_select_desc;
-int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab);
+int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab, int is_f32);
 int mmf_beam_select(const mmf_beam_select_desc* d, void* stream);
 /* Tables after a selection: row w of a group becomes row parents[w]; the first child of a row keeps its unfinished block's page, every other child gets the page
  * of a row without children and a line in copies [groups * beams, 3] (source, destination, tokens; else -1) for mmf_paged_copy.  tables_out may be tables. */

@@ -244,7 +244,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
         o[3] = c.take({G, W}, at::kBool);
         if (history.defined()) o[4] = at::empty(history.sizes(), history.options());
     }
-    const Tensor ws = workspace(mmf_beam_select_ws_bytes((int)G, (int)W, V), logits);
+    const Tensor ws = workspace(mmf_beam_select_ws_bytes((int)G, (int)W, V, logits.scalar_type() == at::kFloat), logits);
     mmf_beam_select_desc d = {};
     d.logits = P(logits); d.ld = G * W == 1 ? V : logits.stride(0);
     d.scores = PT<float>(scores); d.finished = PT<uint8_t>(finished); d.history = PT<int64_t>(history);

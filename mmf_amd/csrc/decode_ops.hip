@@ -239,27 +239,44 @@ __global__ __launch_bounds__(256) void paged_write_kernel(mmf_paged_write_desc d
 // end token at score[w].  The W largest, the lowest flat index w * V + v first among equals.  Values of different beams meet in 64 bits:
 // in 32 the sum would round candidates together that are apart.
 //
-// Within a row the order is the logits' own, so a first kernel takes every row in segments, a workgroup each, and leaves the segment's maximum, its sum of exponentials
-// and its W largest; a second one merges the segments and beams of a group.  Both pick W out of N in the same way: the W-th largest of a wave's 64 lane
-// maxima is a bar that at least W values reach, and few more do; those are ranked by counting.  The second look at a segment comes from the caches.
-// Loops stay rolled: a launch that runs its code once waits for the instructions more than for anything else.
+// Within a row the order is the logits' own, so a first kernel takes every row in segments, a workgroup each with the segment in its registers, and leaves the segment's
+// maximum, its sum of exponentials and its W largest; a second one merges the segments and beams of a group.  Both pick W out of N in the same way: of the maxima of
+// 64 groups of threads the W-th largest is a bar that at least W values reach, and few more do; those are ranked by counting.
 // ------------------------------------------------------------------------------------------------
 constexpr double NEG_INF = -__builtin_huge_val();
-constexpr int SEG_MAX = 8192, LIST = 1024;
+constexpr int CHUNKS = 4, LIST = 1024;                            // 16-byte pieces of a segment per thread
+template <typename T> constexpr int seg_max = 256 * CHUNKS * 16 / (int)sizeof(T);
 
 struct Picked { float v; int i; };                                // i: index in the row, -1: none
 struct Segment { double sum; float top; int pad; };               // sum of exp(x - top)
 DEVI bool better(double av, int64_t ai, double bv, int64_t bi) { return av > bv || (av == bv && ai < bi); }
 
-// the W-th largest of a wave's 64 values
-DEVI float wave_bar(float mine, int W, int lane) {
+// The W-th largest of the maxima of 64 groups of four threads; `top` gets the largest.  Every wave ranks all 64 among 16 of them
+struct Bar { float4 best[16]; int rank[4][64]; float top[4]; };
+DEVI float bar_of(float mine, int W, Bar& b, float& top) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    mine = fmaxf(mine, __shfl_xor(mine, 1, 64));
+    mine = fmaxf(mine, __shfl_xor(mine, 2, 64));
+    float* best = reinterpret_cast<float*>(b.best);
+    if ((tid & 3) == 0) best[tid >> 2] = mine;
+    __syncthreads();
+    const float x = best[lane];
+    const int from = lane - 16 * wave;
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) {
-        const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), j));
-        rank += x > mine || (x == mine && j < lane);
+    float most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float4 y = b.best[4 * wave + j];
+        most = fmaxf(most, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+        rank += (y.x > x || (y.x == x && 4 * j < from)) + (y.y > x || (y.y == x && 4 * j + 1 < from)) + (y.z > x || (y.z == x && 4 * j + 2 < from)) +
+                (y.w > x || (y.w == x && 4 * j + 3 < from));
     }
-    return __shfl(mine, __ffsll((unsigned long long)__ballot(rank == W - 1)) - 1, 64);
+    b.rank[wave][lane] = rank;
+    if (lane == 0) b.top[wave] = most;
+    __syncthreads();
+    rank = b.rank[0][lane] + b.rank[1][lane] + b.rank[2][lane] + b.rank[3][lane];
+    top = fmaxf(fmaxf(b.top[0], b.top[1]), fmaxf(b.top[2], b.top[3]));
+    return __shfl(x, __ffsll((unsigned long long)__ballot(rank == W - 1)) - 1, 64);
 }
 
 // exp(x) for x <= 0, the rounding of x log2 e carried along: relative 2^-23 at any x
@@ -280,29 +297,28 @@ DEVI double log_of(double x) {
     return 2.0 * s * p + e * 0.69314718055994530942;
 }
 
-// 16 bytes of a row as floats; WIDE: rows start on 4 bytes, else on an element.  (NaN loses every comparison and maximum below, as -inf does.)
-template <typename T, bool WIDE> struct Reader {
+// 16 bytes of a row; WIDE: rows start on 4 bytes, else on an element.  Behind the end: -inf.  (NaN loses every comparison and maximum below, as -inf does.)
+template <typename T, bool WIDE> struct Piece {
     static constexpr int VEC = 16 / (int)sizeof(T);
     typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(4)));
-    DEVI static void load(const T* x, int at, int n, float (&v)[VEC]) {
-        T raw[VEC];
+    T x[VEC];
+    DEVI void load(const T* row, int at, int n) {
         if (WIDE && at + VEC <= n) {
-            const u32x4a w = *reinterpret_cast<const u32x4a*>(x + at);
-            __builtin_memcpy(raw, &w, 16);
+            const u32x4a w = *reinterpret_cast<const u32x4a*>(row + at);
+            __builtin_memcpy(x, &w, 16);
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) raw[e] = at + e < n ? x[at + e] : (T)-INFINITY;
+            for (int e = 0; e < VEC; ++e) x[e] = at + e < n ? row[at + e] : (T)-INFINITY;
         }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = (float)raw[e];
     }
 };
 
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void beam_rows_kernel(mmf_beam_select_desc d, int segments, int length) {
-    typedef Reader<T, WIDE> R;
-    constexpr int VEC = R::VEC;
-    __shared__ float cand_v[LIST], tops[4], bars[4];
+    typedef Piece<T, WIDE> P;
+    constexpr int VEC = P::VEC;
+    __shared__ Bar maxima;
+    __shared__ float cand_v[LIST];
     __shared__ int cand_i[LIST], count;
     __shared__ double sums[4];
     const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W = d.beams;
@@ -312,39 +328,39 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(mmf_beam_select_desc d, 
     const int n = (int)min((int64_t)length, d.vocab - first);
     const T* x = (const T*)d.logits + (int64_t)row * d.ld + first;
     if (tid == 0) count = 0;
+    P p[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+        if (c == 0 || 256 * VEC * c < n) p[c].load(x, (256 * c + tid) * VEC, n);
     float mine = -INFINITY;
-#pragma unroll 4
-    for (int at = tid * VEC; at < n; at += 256 * VEC) {
-        float v[VEC];
-        R::load(x, at, n, v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) mine = fmaxf(mine, v[e]);
-    }
-    const float b = wave_bar(mine, W, lane), t = wave_max(mine);
-    if (lane == 0) { tops[wave] = t; bars[wave] = b; }
-    __syncthreads();
-    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const float bar = fmaxf(fmaxf(bars[0], bars[1]), fmaxf(bars[2], bars[3]));
-    const float base = top > -INFINITY && top < INFINITY ? top : 0.f;
+    for (int c = 0; c < CHUNKS; ++c)
+        if (c == 0 || 256 * VEC * c < n)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) mine = fmaxf(mine, (float)p[c].x[e]);
+    float top;
+    const float bar = bar_of(mine, W, maxima, top), base = top > -INFINITY && top < INFINITY ? top : 0.f;
     double s = 0.0;
-#pragma unroll 2
-    for (int at = tid * VEC; at < n; at += 256 * VEC) {
-        float v[VEC];
-        R::load(x, at, n, v);
-        bool any = false;
 #pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-            s += (double)((exp_down(v[e] - base) + exp_down(v[e + 1] - base)) + (exp_down(v[e + 2] - base) + exp_down(v[e + 3] - base)));
-            any |= fmaxf(fmaxf(v[e], v[e + 1]), fmaxf(v[e + 2], v[e + 3])) >= bar;
+    for (int c = 0; c < CHUNKS; ++c)
+        if (c == 0 || 256 * VEC * c < n) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4)
+                s += (double)((exp_down((float)p[c].x[e] - base) + exp_down((float)p[c].x[e + 1] - base)) +
+                              (exp_down((float)p[c].x[e + 2] - base) + exp_down((float)p[c].x[e + 3] - base)));
         }
-        if (any) {
+    if (mine >= bar && mine > -INFINITY) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (v[e] >= bar && v[e] > -INFINITY) {
-                    const int to = atomicAdd(&count, 1);
-                    if (to < LIST) { cand_v[to] = v[e]; cand_i[to] = at + e; }
+        for (int c = 0; c < CHUNKS; ++c)
+            if (c == 0 || 256 * VEC * c < n)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float y = (float)p[c].x[e];
+                    if (y >= bar && y > -INFINITY) {
+                        const int to = atomicAdd(&count, 1);
+                        if (to < LIST) { cand_v[to] = y; cand_i[to] = (256 * c + tid) * VEC + e; }
+                    }
                 }
-        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -400,7 +416,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     __shared__ double cand_v[LIST], score[MMF_BEAMS_MAX], lse[MMF_BEAMS_MAX], best_v[MMF_BEAMS_MAX], red_v[4];
     __shared__ int64_t cand_i[LIST], best_i[MMF_BEAMS_MAX], red_i[4];
     __shared__ int done[MMF_BEAMS_MAX], parent[MMF_BEAMS_MAX], count;
-    __shared__ float bars[4];
+    __shared__ Bar maxima;
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W = d.beams;
     const int64_t V = d.vocab;
     const Picked* picked = (const Picked*)d.ws + (int64_t)g * W * segments * W;
@@ -414,24 +430,21 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     }
     if (tid == 0) count = 0;
     __syncthreads();
-#pragma unroll 1
-    for (int w = wave; w < W; w += 4) {                           // lse: NaN marks a row without candidates
-        if (done[w] || !(score[w] > NEG_INF)) {
-            if (lane == 0) lse[w] = __builtin_nan("");
-            continue;
-        }
+    for (int w0 = 0; w0 < W; w0 += 16) {                          // lse, by 16 lanes each: NaN marks a row without candidates
+        const int w = w0 + (tid >> 4), l16 = tid & 15;
+        const bool live = w < W && !done[w] && score[w] > NEG_INF;
         float m = -INFINITY;
-        for (int s = lane; s < segments; s += 64) m = fmaxf(m, segs[w * segments + s].top);
-        m = wave_max(m);
+        for (int s = live ? l16 : segments; s < segments; s += 16) m = fmaxf(m, segs[w * segments + s].top);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
         double sum = 0.0;
-        for (int s = lane; s < segments; s += 64) {
+        for (int s = live ? l16 : segments; s < segments; s += 16) {
             const Segment x = segs[w * segments + s];
             if (x.top > -INFINITY) sum += x.sum * (double)exp_down(x.top - m);
         }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        const double z = log_of(sum);
-        if (lane == 0) lse[w] = m > -INFINITY && m < INFINITY ? (double)m + z : __builtin_nan("");
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (l16 == 0 && w < W) lse[w] = live && m > -INFINITY && m < INFINITY ? (double)m + log_of(sum) : __builtin_nan("");
     }
     __syncthreads();
     // candidate k of beam w's lists; a finished beam's only one stands first in its lists
@@ -447,21 +460,23 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
         }
         return v;
     };
+    const float one = 1.f / per;                                  // k / per for k < 2^20: half a unit is more than the rounding
+    auto beam_of = [&](int k) { return (int)(((float)k + 0.5f) * one); };
     float mine = -INFINITY;                                       // (rounding to 32 bits keeps the order)
-#pragma unroll 1
+#pragma unroll 4
     for (int k = tid; k < W * per; k += 256) {
         int64_t i;
-        mine = fmaxf(mine, (float)cand(k / per, k % per, i));
+        const int w = beam_of(k);
+        mine = fmaxf(mine, (float)cand(w, k - w * per, i));
     }
-    const float b = wave_bar(mine, W, lane);
-    if (lane == 0) bars[wave] = b;
-    __syncthreads();
-    const float bar = fmaxf(fmaxf(bars[0], bars[1]), fmaxf(bars[2], bars[3]));
-    if (mine >= bar)
+    float top;
+    const float bar = bar_of(mine, W, maxima, top);
+    if (mine >= bar && mine > -INFINITY)
 #pragma unroll 1
         for (int k = tid; k < W * per; k += 256) {
             int64_t i;
-            const double v = cand(k / per, k % per, i);
+            const int w = beam_of(k);
+            const double v = cand(w, k - w * per, i);
             if (v > NEG_INF && (float)v >= bar) {
                 const int to = atomicAdd(&count, 1);
                 if (to < LIST) { cand_v[to] = v; cand_i[to] = i; }
@@ -487,7 +502,8 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
 #pragma unroll 1
             for (int k = tid; k < W * per; k += 256) {
                 int64_t i;
-                const double v = cand(k / per, k % per, i);
+                const int w = beam_of(k);
+                const double v = cand(w, k - w * per, i);
                 if (v > NEG_INF && better(last, last_i, v, i) && better(v, i, bv, bi)) { bv = v; bi = i; }
             }
 #pragma unroll 1
@@ -520,7 +536,8 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     __syncthreads();
     if (tid < W) {
         const int64_t i = best_i[tid];
-        const int p = (int)(i / V);
+        int p = 0;
+        while ((p + 1) * V <= i) ++p;
         const int64_t token = i - p * V;
         parent[tid] = p;
         best_i[tid] = token;
@@ -532,16 +549,19 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     __syncthreads();
     if (!d.history) return;
     const int64_t at = (int64_t)g * W * d.length;
-    const int cols = LIST / W;                                    // through LDS, many columns at a time: in place as well
+    const int cols = (int)min((int64_t)(LIST / W), d.length);     // through LDS, many columns at a time: in place as well
+    const float per_col = 1.f / cols;
     for (int64_t t0 = 0; t0 < d.length; t0 += cols) {
+#pragma unroll 4
         for (int k = tid; k < W * cols; k += 256) {
-            const int w = k / cols;
+            const int w = (int)(((float)k + 0.5f) * per_col);
             const int64_t t = t0 + k - w * cols;
             if (t < d.length) cand_i[k] = t == d.step ? best_i[w] : d.history[at + parent[w] * d.length + t];
         }
         __syncthreads();
+#pragma unroll 4
         for (int k = tid; k < W * cols; k += 256) {
-            const int w = k / cols;
+            const int w = (int)(((float)k + 0.5f) * per_col);
             const int64_t t = t0 + k - w * cols;
             if (t < d.length) d.history_out[at + w * d.length + t] = cand_i[k];
         }
@@ -549,9 +569,10 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     }
 }
 
-// Segments of a row: up to 8192 values, and shorter ones where few rows would leave compute units idle (four workgroups for each), down to 1024 values
-int beam_segments(int rows, int64_t vocab, int* length) {
-    const int64_t least = (vocab + SEG_MAX - 1) / SEG_MAX, fill = (1024 + rows - 1) / rows, most = vocab / 1024;
+// Segments of a row: as long as a workgroup holds, and shorter where few rows would leave compute units idle (four workgroups for each), down to a piece per thread
+int beam_segments(int rows, int64_t vocab, bool f32, int* length) {
+    const int64_t least = (vocab + (f32 ? seg_max<float> : seg_max<bf16>) - 1) / (f32 ? seg_max<float> : seg_max<bf16>), fill = (1024 + rows - 1) / rows;
+    const int64_t most = vocab / (f32 ? 1024 : 2048);
     int64_t n = fill < most ? fill : most;
     if (n < least) n = least;
     const int64_t len = ((vocab + n - 1) / n + 7) / 8 * 8;
@@ -692,10 +713,10 @@ int mmf_paged_write(const mmf_paged_write_desc* d, void* stream) {
     return 0;
 }
 
-int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab) {
+int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab, int is_f32) {
     if (groups < 1 || beams < 1 || vocab < 1) return 0;
     int length;
-    const int64_t rows = (int64_t)groups * beams, n = beam_segments((int)rows, vocab, &length);
+    const int64_t rows = (int64_t)groups * beams, n = beam_segments((int)rows, vocab, is_f32 != 0, &length);
     return ((rows * n * beams + 1) & ~1ll) * (int64_t)sizeof(Picked) + rows * n * (int64_t)sizeof(Segment);
 }
 
@@ -706,7 +727,7 @@ int mmf_beam_select(const mmf_beam_select_desc* d, void* stream) {
     MMF_CHECK_ARG(d->eos >= 0 && d->eos < d->vocab, "beam_select: the end token is not in the vocabulary");
     MMF_CHECK_ARG(!d->history || (d->history_out && d->length > 0 && d->step >= 0 && d->step < d->length), "beam_select: step is not a column of the history");
     int length;
-    const int segments = beam_segments(d->groups * d->beams, d->vocab, &length);
+    const int segments = beam_segments(d->groups * d->beams, d->vocab, d->is_f32 != 0, &length);
     const dim3 grid(segments, d->groups * d->beams);
     const bool wide = ((uintptr_t)d->logits & 3) == 0 && (d->ld & 1) == 0;
     if (d->is_f32) hipLaunchKernelGGL((beam_rows_kernel<float, true>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
