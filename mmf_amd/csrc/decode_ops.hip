@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(mmf_paged_write_desc d
 // 64 groups of threads the W-th largest is a bar that at least W values reach, and few more do; those are ranked by counting.
 // ------------------------------------------------------------------------------------------------
 constexpr double NEG_INF = -__builtin_huge_val();
-constexpr int CHUNKS = 4, LIST = 1024;                            // 16-byte pieces of a segment per thread
+constexpr int CHUNKS = 4, LIST = 1024, KEEP = LIST / 256;                            // 16-byte pieces of a segment per thread
 template <typename T> constexpr int seg_max = 256 * CHUNKS * 16 / (int)sizeof(T);
 
 struct Picked { float v; int i; };                                // i: index in the row, -1: none
@@ -292,7 +292,7 @@ DEVI double log_of(double x) {
     if (m < 0.70710678118654752) { m *= 2.0; e -= 1; }
     const double s = (m - 1.0) / (m + 1.0), q = s * s;
     double p = 1.0 / 15.0;
-#pragma unroll 1
+#pragma unroll
     for (int k = 13; k >= 1; k -= 2) p = p * q + 1.0 / k;
     return 2.0 * s * p + e * 0.69314718055994530942;
 }
@@ -314,7 +314,7 @@ template <typename T, bool WIDE> struct Piece {
 };
 
 template <typename T, bool WIDE>
-__global__ __launch_bounds__(256) void beam_rows_kernel(mmf_beam_select_desc d, int segments, int length) {
+__global__ __launch_bounds__(256, WIDE ? 8 : 4) void beam_rows_kernel(mmf_beam_select_desc d, int segments, int length) {
     typedef Piece<T, WIDE> P;
     constexpr int VEC = P::VEC;
     __shared__ Bar maxima;
@@ -429,6 +429,23 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
         best_i[tid] = -1;
     }
     if (tid == 0) count = 0;
+    const int per = segments * W, cols = (int)min((int64_t)(LIST / W), d.length);
+    const float one = 1.f / per, per_col = 1.f / cols;            // k / per for k < 2^20: half a unit is more than the rounding
+    auto beam_of = [&](int k) { return (int)(((float)k + 0.5f) * one); };
+    const int64_t at = (int64_t)g * W * d.length;
+    Picked early[KEEP];                                           // what does not wait for the sums
+    int64_t past[KEEP];
+#pragma unroll
+    for (int e = 0; e < KEEP; ++e) {
+        const int k = tid + 256 * e;
+        early[e] = Picked{-INFINITY, -1};
+        past[e] = 0;
+        if (k < W * per) early[e] = picked[k];
+        if (d.history && k < W * cols) {
+            const int w = (int)(((float)k + 0.5f) * per_col);
+            past[e] = d.history[at + w * d.length + k - w * cols];
+        }
+    }
     __syncthreads();
     for (int w0 = 0; w0 < W; w0 += 16) {                          // lse, by 16 lanes each: NaN marks a row without candidates
         const int w = w0 + (tid >> 4), l16 = tid & 15;
@@ -448,40 +465,46 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     }
     __syncthreads();
     // candidate k of beam w's lists; a finished beam's only one stands first in its lists
-    const int per = segments * W;
-    auto cand = [&](int w, int k, int64_t& i) {
+    auto cand = [&](int k, const Picked& p, int64_t& i) {
+        const int w = beam_of(k);
         double v = NEG_INF;
         i = w * V;
         if (done[w]) {
-            if (k == 0) { v = score[w]; i += d.eos; }
-        } else if (lse[w] == lse[w]) {
-            const Picked p = picked[w * per + k];
-            if (p.i >= 0) { v = score[w] + ((double)p.v - lse[w]); i += p.i; }
-        }
+            if (k == w * per) { v = score[w]; i += d.eos; }
+        } else if (lse[w] == lse[w] && p.i >= 0) { v = score[w] + ((double)p.v - lse[w]); i += p.i; }
         return v;
     };
-    const float one = 1.f / per;                                  // k / per for k < 2^20: half a unit is more than the rounding
-    auto beam_of = [&](int k) { return (int)(((float)k + 0.5f) * one); };
     float mine = -INFINITY;                                       // (rounding to 32 bits keeps the order)
+    int64_t at_i[KEEP];
+    double at_v[KEEP];
+#pragma unroll
+    for (int e = 0; e < KEEP; ++e) {
+        at_v[e] = tid + 256 * e < W * per ? cand(tid + 256 * e, early[e], at_i[e]) : NEG_INF;
+        mine = fmaxf(mine, (float)at_v[e]);
+    }
 #pragma unroll 4
-    for (int k = tid; k < W * per; k += 256) {
+    for (int k = tid + 256 * KEEP; k < W * per; k += 256) {
         int64_t i;
-        const int w = beam_of(k);
-        mine = fmaxf(mine, (float)cand(w, k - w * per, i));
+        mine = fmaxf(mine, (float)cand(k, picked[k], i));
     }
     float top;
     const float bar = bar_of(mine, W, maxima, top);
-    if (mine >= bar && mine > -INFINITY)
-#pragma unroll 1
-        for (int k = tid; k < W * per; k += 256) {
-            int64_t i;
-            const int w = beam_of(k);
-            const double v = cand(w, k - w * per, i);
-            if (v > NEG_INF && (float)v >= bar) {
-                const int to = atomicAdd(&count, 1);
-                if (to < LIST) { cand_v[to] = v; cand_i[to] = i; }
-            }
+    auto keep = [&](double v, int64_t i) {
+        if (v > NEG_INF && (float)v >= bar) {
+            const int to = atomicAdd(&count, 1);
+            if (to < LIST) { cand_v[to] = v; cand_i[to] = i; }
         }
+    };
+    if (mine >= bar && mine > -INFINITY) {
+#pragma unroll
+        for (int e = 0; e < KEEP; ++e) keep(at_v[e], at_i[e]);
+#pragma unroll 1
+        for (int k = tid + 256 * KEEP; k < W * per; k += 256) {
+            int64_t i;
+            const double v = cand(k, picked[k], i);
+            keep(v, i);
+        }
+    }
     __syncthreads();
     const int found = count;
     if (found <= LIST) {
@@ -502,8 +525,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
 #pragma unroll 1
             for (int k = tid; k < W * per; k += 256) {
                 int64_t i;
-                const int w = beam_of(k);
-                const double v = cand(w, k - w * per, i);
+                const double v = cand(k, picked[k], i);
                 if (v > NEG_INF && better(last, last_i, v, i) && better(v, i, bv, bi)) { bv = v; bi = i; }
             }
 #pragma unroll 1
@@ -548,22 +570,26 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     }
     __syncthreads();
     if (!d.history) return;
-    const int64_t at = (int64_t)g * W * d.length;
-    const int cols = (int)min((int64_t)(LIST / W), d.length);     // through LDS, many columns at a time: in place as well
-    const float per_col = 1.f / cols;
+    // through LDS, many columns at a time: in place as well
+#pragma unroll
+    for (int e = 0; e < KEEP; ++e)
+        if (tid + 256 * e < W * cols) cand_i[tid + 256 * e] = past[e];
+    __syncthreads();
     for (int64_t t0 = 0; t0 < d.length; t0 += cols) {
+        if (t0) {
 #pragma unroll 4
-        for (int k = tid; k < W * cols; k += 256) {
-            const int w = (int)(((float)k + 0.5f) * per_col);
-            const int64_t t = t0 + k - w * cols;
-            if (t < d.length) cand_i[k] = t == d.step ? best_i[w] : d.history[at + parent[w] * d.length + t];
+            for (int k = tid; k < W * cols; k += 256) {
+                const int w = (int)(((float)k + 0.5f) * per_col);
+                const int64_t t = t0 + k - w * cols;
+                if (t < d.length) cand_i[k] = d.history[at + w * d.length + t];
+            }
+            __syncthreads();
         }
-        __syncthreads();
 #pragma unroll 4
         for (int k = tid; k < W * cols; k += 256) {
             const int w = (int)(((float)k + 0.5f) * per_col);
             const int64_t t = t0 + k - w * cols;
-            if (t < d.length) d.history_out[at + w * d.length + t] = cand_i[k];
+            if (t < d.length) d.history_out[at + w * d.length + t] = t == d.step ? best_i[w] : cand_i[parent[w] * cols + k - w * cols];
         }
         __syncthreads();
     }
