@@ -83,24 +83,22 @@ template <int ROWS> DEVI int page_of(const Args& a, const int32_t* table, int ke
     return table[max(min(key0 + (lane & (ROWS - 1)), end - 1), 0) >> a.page_shift];
 }
 
-DEVI void pick(f32x16& o, const f32x16& x, bool take) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[r] = take ? x[r] : o[r];
-}
-
-// ---- the rows of a wave: their queries, and the operands of a tile of NS x 32 keys as the two products take them ----
+// ---- the rows of a wave: their queries, and the operands of a tile of 32 keys as the two products take them ----
 // A tile's operands are all read before the first product that needs them: keys, then the score products; values, which land while the softmax is worked out, then
 // the products that add them up.  Left to itself the compiler reads each operand right before its product, and waits for LDS 32 times a tile.
-template <typename T, int D, int NS> struct Operands;
+//
+// A key that a row does not see adds 0 * v to it, which is 0 unless v is an infinity or no number.  Where the rows of a tile see different keys its values are looked
+// through for those; zeros take their place, and once all tiles are added up they are added to the rows that see them, from the cache (add_odd).
+DEVI int key_of(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }        // the key of a lane's score r
+
+template <typename T, int D> struct Operands;
 template <typename T, int D> struct Rows;
 
-template <int D, int NS> struct Operands<bf16, D, NS> {
-    bf16x8 k[NS][D / 16], v[2 * NS][D / 32];
+template <int D> struct Operands<bf16, D> {
+    bf16x8 k[D / 16], v[2][D / 32];
     DEVI void read_k(const unsigned char* img, int lane) {
 #pragma unroll
-        for (int u = 0; u < D / 16; ++u)
-#pragma unroll
-            for (int n = 0; n < NS; ++n) k[n][u] = *reinterpret_cast<const bf16x8*>(img + at<2 * D>(32 * n + (lane & 31), 2 * u + (lane >> 5)));
+        for (int u = 0; u < D / 16; ++u) k[u] = *reinterpret_cast<const bf16x8*>(img + at<2 * D>(lane & 31, 2 * u + (lane >> 5)));
     }
     // V^T by ds_read_b64_tr_b16 (16 lanes read 4 rows x 16 columns, lane i gets column i): step u takes keys 16 u .. + 16 in the order that a lane holds their scores.
     DEVI void read_v(const unsigned char* img, int lane) {
@@ -108,7 +106,7 @@ template <int D, int NS> struct Operands<bf16, D, NS> {
         typedef short s16x8 __attribute__((ext_vector_type(8)));
         const int g = lane >> 4, i = lane & 15;
 #pragma unroll
-        for (int u = 0; u < 2 * NS; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int t = 0; t < D / 32; ++t) {
                 const int row = 16 * u + 4 * (g >> 1) + (i >> 2), col = 32 * t + 16 * (g & 1) + (i & 3) * 4;
@@ -116,6 +114,32 @@ template <int D, int NS> struct Operands<bf16, D, NS> {
                 const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(img + at<2 * D>(row + 8, col >> 3) + (col & 7) * 2));
                 const s16x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                 v[u][t] = __builtin_bit_cast(bf16x8, x);
+            }
+    }
+    DEVI bool odd() const {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 most = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, __builtin_bit_cast(u32x4, v[u][t])[e] & 0x7fff7fffu));
+        return __ballot(most[0] >= 0x7f80 || most[1] >= 0x7f80) != 0;
+    }
+    DEVI void clear_odd() {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) {
+                u32x4 w = __builtin_bit_cast(u32x4, v[u][t]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0x0000ffffu;
+                    if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+                }
+                v[u][t] = __builtin_bit_cast(bf16x8, w);
+                __builtin_amdgcn_sched_barrier(0);
             }
     }
 };
@@ -129,54 +153,56 @@ template <int D> struct Rows<bf16, D> {
             q[s] = __builtin_bit_cast(bf16x8, (x & a.q_and) ^ (a.q_xor | a.q_xor >> 16));
         }
     }
-    template <int NS> DEVI void scores(const Operands<bf16, D, NS>& x, f32x16 (&s)[NS]) const {
+    DEVI void scores(const Operands<bf16, D>& x, f32x16& s) const {
 #pragma unroll
-        for (int u = 0; u < D / 16; ++u)
-#pragma unroll
-            for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.k[n][u], q[u], s[n], 0, 0, 0);
+        for (int u = 0; u < D / 16; ++u) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.k[u], q[u], s, 0, 0, 0);
     }
-    // sums += V^T p (PICK: in the lanes that `take`; a value that is no number stays with them).  p is rounded to bf16: relative 2^-8 of each, the pool's own precision.
-    template <int NS, bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16 (&p)[NS], const Operands<bf16, D, NS>& x, bool take) {
-        bf16x8 pb[2 * NS];
+    // sums += V^T p.  p is rounded to bf16: relative 2^-8 of each, the pool's own precision.
+    DEVI static void add(f32x16 (&o)[D / 32], const f32x16& p, const Operands<bf16, D>& x) {
+        bf16x8 pb[2];
 #pragma unroll
-        for (int u = 0; u < 2 * NS; ++u)
+        for (int r = 0; r < 16; ++r) pb[r >> 3][r & 7] = (bf16)p[r];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pb[u][e] = (bf16)p[u >> 1][8 * (u & 1) + e];
-        if (PICK) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int t = 0; t < D / 32; ++t) {
-                f32x16 acc = o[t];
-#pragma unroll
-                for (int u = 0; u < 2 * NS; ++u) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[u][t], pb[u], acc, 0, 0, 0);
-                pick(o[t], acc, take);
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < 2 * NS; ++u)
-#pragma unroll
-                for (int t = 0; t < D / 32; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[u][t], pb[u], o[t], 0, 0, 0);
-        }
+            for (int t = 0; t < D / 32; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[u][t], pb[u], o[t], 0, 0, 0);
     }
 };
 
 // fp32: a step of v_mfma_f32_32x32x2_f32 takes one element per lane, lanes 0 - 31 of reduction slot 0 and lanes 32 - 63 of slot 1
-template <int D, int NS> struct Operands<float, D, NS> {
-    f32x4 k[NS][D / 8];                                            // element (t, e) of half h: column 8 t + 4 h + e
-    float v[16 * NS][D / 32];                                      // step r of half h: key 8 (r / 4) + 4 h + r % 4, as a lane holds the scores
+template <int D> struct Operands<float, D> {
+    f32x4 k[D / 8];                                                // element (t, e) of half h: column 8 t + 4 h + e
+    float v[16][D / 32];                                           // step r: key_of(r), as a lane holds the scores
     DEVI void read_k(const unsigned char* img, int lane) {
 #pragma unroll
-        for (int t = 0; t < D / 8; ++t)
-#pragma unroll
-            for (int n = 0; n < NS; ++n) k[n][t] = *reinterpret_cast<const f32x4*>(img + at<4 * D>(32 * n + (lane & 31), 2 * t + (lane >> 5)));
+        for (int t = 0; t < D / 8; ++t) k[t] = *reinterpret_cast<const f32x4*>(img + at<4 * D>(lane & 31, 2 * t + (lane >> 5)));
     }
     DEVI void read_v(const unsigned char* img, int lane) {
 #pragma unroll
-        for (int r = 0; r < 16 * NS; ++r)
+        for (int r = 0; r < 16; ++r)
 #pragma unroll
             for (int t = 0; t < D / 32; ++t) {
-                const int row = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), col = 32 * t + (lane & 31);
-                v[r][t] = *reinterpret_cast<const float*>(img + at<4 * D>(row, col >> 2) + (col & 3) * 4);
+                const int col = 32 * t + (lane & 31);
+                v[r][t] = *reinterpret_cast<const float*>(img + at<4 * D>(key_of(r, lane), col >> 2) + (col & 3) * 4);
             }
+    }
+    DEVI bool odd() const {
+        float most = 0.f;
+        bool none = false;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) {
+                none |= v[r][t] != v[r][t];
+                most = fmaxf(most, fabsf(v[r][t]));
+            }
+        return __ballot(none || most == INFINITY) != 0;
+    }
+    DEVI void clear_odd() {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) v[r][t] = fabsf(v[r][t]) < INFINITY ? v[r][t] : 0.f;
     }
 };
 template <int D> struct Rows<float, D> {
@@ -189,31 +215,35 @@ template <int D> struct Rows<float, D> {
             q[t] = __builtin_bit_cast(f32x4, (x & a.q_and) ^ a.q_xor);
         }
     }
-    template <int NS> DEVI void scores(const Operands<float, D, NS>& x, f32x16 (&s)[NS]) const {
+    DEVI void scores(const Operands<float, D>& x, f32x16& s) const {
 #pragma unroll
         for (int t = 0; t < D / 8; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.k[n][t][e], q[t][e], s[n], 0, 0, 0);
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.k[t][e], q[t][e], s, 0, 0, 0);
     }
-    template <int NS, bool PICK> DEVI static void add(f32x16 (&o)[D / 32], const f32x16 (&p)[NS], const Operands<float, D, NS>& x, bool take) {
-        if (PICK) {
+    DEVI static void add(f32x16 (&o)[D / 32], const f32x16& p, const Operands<float, D>& x) {
 #pragma unroll
-            for (int t = 0; t < D / 32; ++t) {
-                f32x16 acc = o[t];
+        for (int r = 0; r < 16; ++r)
 #pragma unroll
-                for (int r = 0; r < 16 * NS; ++r) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[r][t], p[r >> 4][r & 15], acc, 0, 0, 0);
-                pick(o[t], acc, take);
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 16 * NS; ++r)
-#pragma unroll
-                for (int t = 0; t < D / 32; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[r][t], p[r >> 4][r & 15], o[t], 0, 0, 0);
-        }
+            for (int t = 0; t < D / 32; ++t) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[r][t], p[r], o[t], 0, 0, 0);
     }
 };
+
+// the values of one key that are infinite or no number, to the rows that see it
+template <typename T, int D> DEVI void add_odd(const Args& a, f32x16 (&o)[D / 32], const int32_t* table, int h, int key, bool sees, int lane) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const int page = table[key >> a.page_shift];
+    if ((unsigned)page >= (unsigned)a.d.pages) return;
+    const T* v = (const T*)a.d.v_cache + page * a.d.page_stride + h * a.d.head_stride + (key & (a.d.page_size - 1)) * a.d.pos_stride + 4 * (lane >> 5);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const T4 x = *reinterpret_cast<const T4*>(v + 32 * t + 2 * r);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][r + e] += sees && !(fabsf((float)x[e]) < INFINITY) ? (float)x[e] : 0.f;
+        }
+}
 
 // a value and that of lane ^ 32: v_permlane32_swap_b32 leaves the lower half's in one register and the upper half's in the other (the second copy is kept
 // apart from the first: of two equal operands the compiler returns the first result for both)
@@ -233,18 +263,18 @@ DEVI int wave_min(int v) {
     return __builtin_amdgcn_readfirstlane(v);
 }
 
-// `ahead` is called once the tile's operands are read: loads into LDS that are under way when the transposed values are read would be waited for first.
-// One tile of NS x 32 keys, key0 its first, for the rows of a wave; lim: keys this lane's row sees.  m (in units of log2) may lag up to 8 behind the largest score:
+// One tile of 32 keys, key0 its first, for the rows of a wave; lim: keys this lane's row sees.  m (in units of log2) may lag up to 8 behind the largest score:
 // a probability is then at most 2^8, and the sums need no rescaling on most tiles.
-template <typename T, int D, int NS, bool PICK, typename F>
+// `ahead` is called once the tile's operands are read: loads into LDS that are under way when the transposed values are read would be waited for first.
+template <typename T, int D, typename F>
 DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsigned char* v, int key0, int lim, bool masked, float c, float& m, float& l, f32x16 (&o)[D / 32],
-                    int lane, bool take, F ahead) {
-    f32x16 s[NS] = {};
-    Operands<T, D, NS> x;
+                    int lane, bool& odd, F ahead) {
+    f32x16 s = {};
+    Operands<T, D> x;
     x.read_k(k, lane);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);                                           // a wave at its products goes before one at its softmax
-    rows.template scores<NS>(x, s);
+    rows.scores(x, s);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
     x.read_v(v, lane);
@@ -252,18 +282,14 @@ DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsign
     ahead();
     __builtin_amdgcn_sched_barrier(0);
     float top = -INFINITY;
-    const int h4 = 4 * (lane >> 5);
     if (masked) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (key0 + 32 * n + 8 * (r >> 2) + h4 + (r & 3) >= lim) s[n][r] = -INFINITY;
+        for (int r = 0; r < 16; ++r)
+            if (key0 + key_of(r, lane) >= lim) s[r] = -INFINITY;
+        if (x.odd()) { x.clear_odd(); odd = true; }
     }
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
     top = max_halves(top) * c;
     if (__ballot(top > m + 8.f) != 0) {
         const float next = fmaxf(m, top), keep = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - next);
@@ -277,15 +303,13 @@ DEVI void tile_step(const Rows<T, D>& rows, const unsigned char* k, const unsign
     const float mm = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -mm));
-            sum += s[n][r];
-        }
+    for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mm));
+        sum += s[r];
+    }
     l += sum;
     __builtin_amdgcn_s_setprio(1);
-    Rows<T, D>::template add<NS, PICK>(o, s, x, take);
+    Rows<T, D>::add(o, s, x);
     __builtin_amdgcn_s_setprio(0);
 }
 
@@ -502,6 +526,7 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         const int free_to = wave_min(lim), see_to = -wave_min(row.token >= 0 ? -lim : 0);       // keys that every row of the wave sees, that any does
         const bool idle = row0 + 32 * wave >= x.n * a.group;                     // a wave without rows only helps to stage
         float m = -INFINITY, l = 0.f;
+        bool odd = false;
         f32x16 o[D / 32] = {};
         const int32_t* table = a.d.tables + x.req * a.d.table_row;
         const int64_t head_off = h * a.d.head_stride;
@@ -525,10 +550,15 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
             };
             const int subs = idle ? 0 : (min(min(see_to, end) - key0, KT) + 31) >> 5;
             if (subs <= 0) { ahead(); continue; }
-            { const int n = 0; tile_step<T, D, 1, false>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane, true, ahead); }
-            if (subs == 2) { const int n = 1; tile_step<T, D, 1, false>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane, true, [] {}); }
+            { const int n = 0; tile_step<T, D>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane, odd, ahead); }
+            if (subs == 2) { const int n = 1; tile_step<T, D>(rows, img + n * 32 * RB, img + IMG + n * 32 * RB, key0 + 32 * n, min(lim, end), key0 + 32 * n + 32 > min(free_to, end), a.c, m, l, o, lane, odd, [] {}); }
         }
         l = add_halves(l);
+        if (odd) {                                                               // from the first tile that not every row sees
+            const int mixed = max(min(free_to, end) - start, 0) / 32 * 32 + start;
+#pragma unroll 1
+            for (int key = mixed; key < min(see_to, end); ++key) add_odd<T, D>(a, o, table, h, key, key < lim, lane);
+        }
         if (whole) {
             if (row.token >= 0) {
                 T* out = out_row<T, D>(a, row, h);
@@ -613,6 +643,7 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         };
         auto pages = [&](const Job& b) { return page_of<32>(a, table + max(b.beam, 0) * a.d.table_row, b.key0, b.end, lane); };
         float m = -INFINITY, l = 0.f;
+        bool odd = false;
         f32x16 o[D / 32] = {};
         Job now = job(wave), next = job(wave + 4);
         int page = pages(now), page_next = pages(next);
@@ -629,10 +660,20 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
             };
             const int see = min(lim, now.end);
             const bool take = now.beam < 0 || row.beam == now.beam;              // a tile of one beam: the other beams' rows see none of it
-            tile_step<T, D, 1, true>(rows, mine, mine + IMG, now.key0, take ? see : 0, now.beam >= 0 || now.key0 + 32 > min(free_to, now.end), a.c, m, l, o, lane, take, ahead);
+            tile_step<T, D>(rows, mine, mine + IMG, now.key0, take ? see : 0, now.beam >= 0 || now.key0 + 32 > min(free_to, now.end), a.c, m, l, o, lane, odd, ahead);
             now = next; next = after;
         }
         l = add_halves(l);
+        if (odd) {
+#pragma unroll 1
+            for (int j = wave; j < jobs; j += 4) {
+                const Job b = job(j);
+                if (b.beam < 0 && b.key0 + 32 <= min(free_to, b.end)) continue;
+#pragma unroll 1
+                for (int key = b.key0; key < min(b.key0 + 32, b.end); ++key)
+                    add_odd<T, D>(a, o, table + max(b.beam, 0) * a.d.table_row, h, key, key < lim && (b.beam < 0 || row.beam == b.beam), lane);
+            }
+        }
         // the four waves' sums meet: [wave][row][D] fp32 in the tiles' place, [wave][row][2] behind
         __syncthreads();
         constexpr int LD = D + 4;                                                // (rows of D floats alone would put every row's column on one bank)

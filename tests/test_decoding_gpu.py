@@ -236,6 +236,39 @@ def test_large_scores_and_values(dtype, new):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kv,new,beams,shared,heads,dim", [([70, 33, 90], [40, 33, 7], 1, 0, 4, 64), ([70, 200], [64, 130], 1, 0, 8, 128), ([40, 70, 64], [4, 2, 1], 1, 0, 4, 128),
+                                                          ([70, 50], [1, 1], 4, 48, 2, 64), ([100], [3], 2, 32, 4, 64), ([3000], [50], 1, 0, 2, 64), ([3000], [2], 1, 0, 2, 128)])
+def test_infinities_and_nan_stay_with_the_rows_that_see_them(dtype, kv, new, beams, shared, heads, dim):
+    """Values (of later tokens in the chunk, of another beam, of an early key) that are infinite or no number: a row that sees one has it in its column, every other output
+    is what it was, bit for bit.  A key that is no number: all of a row that sees it, nothing of the others."""
+    c = attend_case(kv, new, beams=beams, heads=heads, kv_heads=2, dim=dim, dtype=dtype, shared=shared)
+    good = attend_check(c, beams=beams)
+
+    def spot(r, key):
+        return int(c["tables"][r, key // 16]), key % 16
+    for cache in ("value_cache", "key_cache"):
+        bad = dict(c, **{cache: c[cache].clone()})
+        for r in range(len(kv) * beams):
+            n, m = kv[r // beams], new[r // beams]
+            for k, (key, col, x) in enumerate([(n - 1, 5, float("nan")), (n - 1, 37, float("inf")), (n - 1 - m // 2, 6, float("-inf")), (n - 1 - m // 2, 37, float("-inf")),
+                                               (max(0, n - m) // 2 + 1, 60, float("inf")), (n - 1 - m // 3, 5, float("inf"))]):
+                if cache == "key_cache" and k > 2:
+                    continue
+                page, pos = spot(r, key)
+                bad[cache][page, r % 2, pos, col] = float("nan") if cache == "key_cache" else x
+        names = ("q", "key_cache", "value_cache", "tables", "kv_lens", "q_start", "q_lens")
+        out = torch.full_like(good, 7.0)
+        got = D().attend_pages(*(bad[k] for k in names), max_q=max(new), beams=beams, out=out)
+        want, _, _, named = O.attend(*(bad[k] for k in names), beams, True, dim ** -0.5)
+        g = got.double().cpu()
+        fine = torch.isfinite(want) & named[:, None, None]
+        assert bool(fine.any()) and not bool(torch.isfinite(want[named]).all())
+        assert torch.equal(g[fine], good.double().cpu()[fine])
+        odd = ~torch.isfinite(want) & named[:, None, None]
+        assert torch.equal(torch.nan_to_num(g[odd], 9.0, 10.0, -10.0), torch.nan_to_num(want[odd], 9.0, 10.0, -10.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_max_q_larger_than_any_request_and_out_in_place_of_q(dtype):
     c = attend_case([90, 40], [9, 20], heads=4, kv_heads=2, dtype=dtype)
     a = attend_check(c, max_q=500)
