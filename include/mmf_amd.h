@@ -805,7 +805,7 @@ int mmf_paged_attention(const mmf_paged_attn_desc* d, void* stream);
 /* The best `beams` continuations of each group over beams x vocabulary (the reference's BeamSearch, mmf/utils/text.py): candidate (w, v) at scores[w] + log_softmax(logits[w])[v], of a finished beam only the
  * end token at scores[w].  Descending; the lowest w * vocab + v first among equals.  NaN logits and scores count as -inf; so does every logit of a row that
  * holds +inf.  finished_out = finished[parent] or token == eos.  history (optional) [groups, beams, length]: rows of the parents, column `step` the new
- * tokens.  Every output may be its input.  logits bf16 or fp32, row stride ld. */
+ * tokens.  Every output may be its input.  logits bf16 or fp32, row stride ld; a vocabulary of up to 2^22. */
 typedef struct mmf_beam_select_desc {
     const void* logits; int64_t ld;
     const float* scores; const uint8_t* finished; const int64_t* history;

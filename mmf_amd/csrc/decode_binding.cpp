@@ -219,7 +219,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
     check_float(logits, "logits");
     NEED(logits.dim() == 2 && logits.size(0) == G * W, "logits must be [", G * W, ", vocab], got ", logits.sizes());
     const int64_t V = logits.size(1);
-    NEED(V > 0 && V <= 0x3fffffff && (logits.stride(1) == 1 || V == 1) && (logits.stride(0) >= V || G * W == 1), "logits must have contiguous rows that do not overlap");
+    NEED(V <= (1 << 22), "a vocabulary of up to 2**22 tokens, got ", V);
+    NEED(V > 0 && (logits.stride(1) == 1 || V == 1) && (logits.stride(0) >= V || G * W == 1), "logits must have contiguous rows that do not overlap");
     check_dense(finished, "finished", at::kBool, {G, W});
     NEED(eos >= 0 && eos < V, "eos ", eos, " is not in the vocabulary of ", V);
     const Tensor history = history_.has_value() ? *history_ : Tensor();

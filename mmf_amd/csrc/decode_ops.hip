@@ -430,7 +430,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     }
     if (tid == 0) count = 0;
     const int per = segments * W, cols = (int)min((int64_t)(LIST / W), d.length);
-    const float one = 1.f / per, per_col = 1.f / cols;            // k / per for k < 2^20: half a unit is more than the rounding
+    const float one = 1.f / per, per_col = 1.f / cols;            // k / per for k < 2^20 (a vocabulary of 2^22): half a unit is more than the rounding
     auto beam_of = [&](int k) { return (int)(((float)k + 0.5f) * one); };
     const int64_t at = (int64_t)g * W * d.length;
     Picked early[KEEP];                                           // what does not wait for the sums
@@ -749,7 +749,7 @@ int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab, int is_f3
 int mmf_beam_select(const mmf_beam_select_desc* d, void* stream) {
     MMF_CHECK_ARG(d && d->logits && d->scores && d->finished && d->scores_out && d->parents && d->tokens && d->finished_out && d->ws, "beam_select: null operand");
     MMF_CHECK_ARG(d->groups > 0 && d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->vocab > 0 && d->ld >= d->vocab, "beam_select: bad shape");
-    MMF_CHECK_ARG(d->vocab <= 0x3fffffff && (int64_t)d->groups * d->beams <= 65535, "beam_select: 2^30 tokens and 65535 rows at most");
+    MMF_CHECK_ARG(d->vocab <= 1 << 22 && (int64_t)d->groups * d->beams <= 65535, "beam_select: 2^22 tokens and 65535 rows at most");
     MMF_CHECK_ARG(d->eos >= 0 && d->eos < d->vocab, "beam_select: the end token is not in the vocabulary");
     MMF_CHECK_ARG(!d->history || (d->history_out && d->length > 0 && d->step >= 0 && d->step < d->length), "beam_select: step is not a column of the history");
     int length;

@@ -66,7 +66,7 @@ def plan_pages(q_lens, kv_lens, tables, owned, free_pages, free_top, *, page_siz
 
 def write_pages(k, v, key_cache, value_cache, slots):
     """k, v [rows, kv_heads, head_dim] (contiguous head_dim; slices of a packed projection as they are) into the slots of their rows: slot = page * page_size +
-    position, negative: the row is left out.  A slot that two rows name gets one of them.  The caches are bf16 or fp32, as k and v."""
+    position, negative: the row is left out.  What a slot holds that two rows name is undefined.  The caches are bf16 or fp32, as k and v."""
     _lib().write_pages(k, v, key_cache, value_cache, slots)
 
 
@@ -85,7 +85,7 @@ def attend_pages(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, *,
 def select_beams(logits, scores, finished, *, eos, history=None, step=0, out=None):
     """The best `beams` continuations of each group over beams x vocabulary.
 
-    logits [groups * beams, vocab] bf16 or fp32 (contiguous rows); scores fp32 [groups, beams]: the sums of log-probabilities so far, -inf for a beam that is not
+    logits [groups * beams, vocab] bf16 or fp32 (contiguous rows; up to 2**22 tokens); scores fp32 [groups, beams]: the sums of log-probabilities so far, -inf for a beam that is not
     live (all but one before the first token); finished bool [groups, beams].  A candidate is scores + log_softmax(logits); a finished beam has one, the token `eos` at its
     score.  Descending, among equals the lowest beam * vocab + token first.  NaN counts as -inf; a row that holds +inf is all -inf.  history int64
     [groups, beams, length]: the rows of the parents come back with the new tokens in column `step`.  `out`: a BeamStep whose tensors take the results; each may be the input

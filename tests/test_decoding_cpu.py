@@ -113,7 +113,7 @@ def test_attend_refuses_head_dims_and_results_it_has_no_kernel_for():
     (dict(), "HBM"), (dict(logits=torch.zeros(5, 10)), "logits"), (dict(logits=torch.zeros(6, 10, dtype=torch.float16)), "logits"), (dict(logits=torch.zeros(10, 6).t()), "contiguous rows"),
     (dict(logits=torch.zeros(10).expand(6, 10)), "overlap"), (dict(scores=torch.zeros(2, 3, dtype=torch.float64)), "scores"), (dict(finished=z(2, 3)), "finished"), (dict(eos=10), "eos"),
     (dict(eos=-1), "eos"), (dict(step=5), "step"), (dict(step=-1), "step"), (dict(history=z(2, 3, 5)), "history"), (dict(history=z(2, 4, 5, dt=I64)), "history"),
-    (dict(scores=torch.zeros(1, 33), logits=torch.zeros(33, 10)), "beams"), (dict(scores=torch.zeros(0, 3), logits=torch.zeros(0, 10)), "group")])
+    (dict(logits=torch.zeros(2 ** 22 + 1).expand(6, -1)), "vocabulary of up to"), (dict(scores=torch.zeros(1, 33), logits=torch.zeros(33, 10)), "beams"), (dict(scores=torch.zeros(0, 3), logits=torch.zeros(0, 10)), "group")])
 def test_select_refuses(over, says):
     a = dict(logits=torch.zeros(6, 10), scores=torch.zeros(2, 3), finished=z(2, 3, dt=torch.bool), eos=2, history=z(2, 3, 5, dt=I64), step=4)
     with pytest.raises(RuntimeError, match=says):

@@ -528,3 +528,111 @@ def test_calls_on_another_stream_than_the_tensors_own():
         got = D().attend_pages(c["q"], c["key_cache"], c["value_cache"], c["tables"], c["kv_lens"], c["q_start"], c["q_lens"], max_q=40)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got[:41], want[:41])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_pages_beyond_32_bits_of_bytes_and_elements(dtype):
+    """A pool whose last pages start behind 2^32 elements: written, read by single tokens and by chunks, copied, as the first pages of a small pool are."""
+    page, heads, dim, near = 64, 8, 128, 40
+    pages = 2 ** 32 // (page * heads * dim) + near
+    pool = torch.empty(2, pages, heads, page, dim, dtype=dtype, device=DEV)
+    small = torch.zeros(2, near, heads, page, dim, dtype=dtype, device=DEV)
+    pool[:, -near:] = 0
+    g = torch.Generator().manual_seed(5)
+    kv = [64 * 9 + 5, 700]
+    k, v = (torch.randn(sum(kv), heads, dim, generator=g).to(dtype).to(DEV) for _ in range(2))
+    tables = torch.randperm(near, generator=g, dtype=I32)[:22].view(2, 11)
+    pos = torch.cat([torch.arange(n) for n in kv])
+    req = torch.repeat_interleave(torch.arange(2), torch.tensor(kv))
+    slots = tables[req, pos // page].long() * page + pos % page
+    far = pages - near
+    D().write_pages(k, v, small[0], small[1], slots.to(DEV))
+    D().write_pages(k, v, pool[0], pool[1], (slots + far * page).to(DEV))
+    assert torch.equal(pool[:, far:], small)
+    for new in ([1, 1], [100, 650]):
+        q = torch.randn(sum(new), 2 * heads, dim, generator=g).to(dtype).to(DEV)
+        rest = dict(kv_lens=i32(kv), q_start=i32([0, new[0]]), q_lens=i32(new), max_q=max(new))
+        assert torch.equal(D().attend_pages(q, pool[0], pool[1], (tables + far).to(DEV), **rest), D().attend_pages(q, small[0], small[1], tables.to(DEV), **rest))
+    D().copy_pages(i32([[int(tables[0, 0]), int(tables[1, 10]), 33]]), small)
+    D().copy_pages(i32([[far + int(tables[0, 0]), far + int(tables[1, 10]), 33]]), pool)
+    assert torch.equal(pool[:, far:], small)
+
+
+@pytest.mark.parametrize("beams,groups,new", [(1, 1000, 1), (1, 1000, 40), (32, 33, 1), (2, 500, 17), (1, 70, 40)])
+def test_more_requests_than_a_launch_takes(beams, groups, new):
+    """Requests beyond what one launch plans for, and beyond those that are put in order of length; each alike: 7 different lengths, compared among themselves and once with the plain form."""
+    kv = [new + (g % 7) * 9 for g in range(groups)]
+    c = attend_case(kv[:7], [new] * 7, beams=beams, heads=2, kv_heads=1)
+    few = attend_check(c, beams=beams)
+    rows, per = new * beams, len(kv[:7])
+    idx = torch.arange(groups, device=DEV) % per
+    many = dict(c, q=c["q"][:rows * per].view(per, rows, 2, 64)[idx].reshape(groups * rows, 2, 64), kv_lens=c["kv_lens"][idx], q_lens=c["q_lens"][idx],
+                tables=c["tables"].view(per, beams, -1)[idx].reshape(groups * beams, -1), q_start=torch.arange(groups * beams, dtype=I32, device=DEV) * new)
+    got = D().attend_pages(many["q"], many["key_cache"], many["value_cache"], many["tables"], many["kv_lens"], many["q_start"], many["q_lens"], max_q=new, beams=beams)
+    assert torch.equal(got.view(groups, rows, 2, 64), few[:rows * per].view(per, rows, 2, 64)[idx])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_select_from_the_largest_vocabulary(dtype):
+    W, V = 32, 2 ** 22
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = (torch.randn(W, V, generator=g, device=DEV) * 2).to(dtype)
+    chosen = torch.randperm(W * V, generator=g, device=DEV)[:W]
+    x.view(-1)[chosen] = (14 + 0.125 * torch.arange(W, device=DEV)).to(dtype)          # (exact in bf16: these and no others are the best)
+    s = torch.zeros(1, W, device=DEV)
+    got = D().select_beams(x, s, torch.zeros(1, W, dtype=torch.bool, device=DEV), eos=0)
+    lse = torch.stack([torch.logsumexp(x[w].double(), 0) for w in range(W)])
+    want, order = (x.view(-1)[chosen].double() - lse[chosen // V]).sort(descending=True)
+    assert float((want[:-1] - want[1:]).min()) > 1e-4
+    assert torch.equal(got.parents[0] * V + got.tokens[0], chosen[order])
+    assert bool(((got.scores[0].double() - want).abs() <= 2.0 ** -22 + 2.0 ** -24 * want.abs() + 2.0 ** -40).all())
+
+
+def test_two_graphs_of_split_attention_replay_in_turn_with_eager_calls_between():
+    """Long caches are split over workgroups and joined through a workspace: two captured calls, and eager ones between their replays, do not meet in it."""
+    cases = [attend_case([3000, 700], [1, 1], heads=4, kv_heads=2, dim=64), attend_case([2500], [60], heads=4, kv_heads=2, dim=64, seed=1)]
+    names = ("q", "key_cache", "value_cache", "tables", "kv_lens", "q_start", "q_lens")
+
+    def call(c):
+        return D().attend_pages(*(c[k] for k in names), max_q=max(1, int(c["q"].shape[0])))
+    for c in cases:
+        call(c)
+    graphs, outs = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(c))
+        graphs.append(g)
+    for turn in range(4):
+        for c in cases:
+            c["q"].copy_(torch.randn(c["q"].shape, generator=torch.Generator().manual_seed(turn)))
+        for i in ((0, 1), (1, 0))[turn & 1]:
+            outs[i].zero_()
+            graphs[i].replay()
+            call(cases[1 - i])
+        torch.cuda.synchronize()
+        for c, o in zip(cases, outs):
+            n = int(c["q_lens"].sum())
+            assert torch.equal(o[:n], call(c)[:n])
+
+
+def test_two_streams_at_once():
+    """Calls that run beside each other: every one has a workspace of its own."""
+    c = [attend_case([3000, 700], [1, 1], heads=4, kv_heads=2, dim=64), attend_case([2500], [60], heads=4, kv_heads=2, dim=64, seed=1)]
+    names = ("q", "key_cache", "value_cache", "tables", "kv_lens", "q_start", "q_lens")
+    x = [torch.randn(8, 5050, device=DEV) for _ in range(2)]
+    s, f = torch.zeros(2, 4, device=DEV), torch.zeros(2, 4, dtype=torch.bool, device=DEV)
+    n = [int(a["q_lens"].sum()) for a in c]
+
+    def run(i):
+        return D().attend_pages(*(c[i][k] for k in names), max_q=60)[:n[i]], *D().select_beams(x[i], s, f, eos=2)[:4]
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, run(i)))
+    torch.cuda.synchronize()
+    for i, r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
