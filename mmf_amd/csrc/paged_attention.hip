@@ -23,7 +23,8 @@ typedef __attribute__((address_space(3))) void* lds_vp;
 typedef const __attribute__((address_space(1))) void* glb_vp;
 static __device__ uint4 g_zero16;
 
-constexpr int STEP_ROWS = 32, CHUNK_ROWS = 128;
+constexpr int STEP_ROWS = 32;
+template <typename T> constexpr int chunk_rows = sizeof(T) == 2 ? 128 : 64;       // a wave per 32
 constexpr int UNITS_MAX = 960;         // requests (chunks) or groups of beams (steps) per launch
 constexpr int PREFIX_MAX = 4 * (UNITS_MAX + 1) * 4;
 
@@ -520,9 +521,9 @@ template <typename T> constexpr int chunk_subtiles = sizeof(T) == 2 ? 2 : 1;    
 template <typename T, int D> constexpr int chunk_lds = 2 * 2 * 32 * chunk_subtiles<T> * D * (int)sizeof(T);
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_attn_chunk_kernel(Args a) {
+__global__ __launch_bounds__(2 * chunk_rows<T>, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_attn_chunk_kernel(Args a) {
     extern __shared__ unsigned char lds[];
-    constexpr int NS = chunk_subtiles<T>, KT = 32 * NS, RB = D * (int)sizeof(T), IMG = KT * RB;
+    constexpr int CHUNK_ROWS = chunk_rows<T>, NW = CHUNK_ROWS / 32, NS = chunk_subtiles<T>, KT = 32 * NS, RB = D * (int)sizeof(T), IMG = KT * RB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Plan plan = make_plan<CHUNK_ROWS>(a, reinterpret_cast<int*>(lds + 4 * IMG));
     for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
         const int32_t* table = a.d.tables + x.req * a.d.table_row;
         const int64_t head_off = h * a.d.head_stride;
         const int steps = end > start ? (end - start + KT - 1) / KT : 0;
-        const Stager<T, D, KT, 4> stage(a, head_off, wave, lane);
+        const Stager<T, D, KT, NW> stage(a, head_off, wave, lane);
         int page = page_of<KT>(a, table, start, end, lane);
         __syncthreads();                                                         // the item before has read its last tile
         if (steps > 0) stage(a, start, end, page, lds, lds + IMG, wave, lane);
@@ -788,11 +789,12 @@ Shape shape_of(const mmf_paged_attn_desc* d) {
     const int64_t rows = (int64_t)d->max_q * (d->heads / d->kv_heads);
     s.chunk = rows > STEP_ROWS;
     s.nb = s.chunk ? 1 : (int)(STEP_ROWS / rows < d->beams ? STEP_ROWS / rows : d->beams);
-    s.target = s.chunk ? 768 : 512;
+    const int tile = !s.chunk ? STEP_ROWS : d->is_f32 ? chunk_rows<float> : chunk_rows<bf16>;
+    s.target = s.chunk ? 768 * 128 / tile : 512;
     s.run_min = s.chunk ? 1024 : 256;
-    s.parts = s.chunk ? 1536 : 1024;
+    s.parts = s.chunk ? 2 * s.target : 1024;
     s.split = (int64_t)d->blocks * d->page_size > s.run_min;
-    s.ws = s.split ? (int64_t)s.parts * (s.chunk ? CHUNK_ROWS : STEP_ROWS) * (d->head_dim + 2) * 4 : 0;
+    s.ws = s.split ? (int64_t)s.parts * tile * (d->head_dim + 2) * 4 : 0;
     return s;
 }
 
@@ -808,6 +810,7 @@ template <typename K> int allow_lds(K* kernel, int bytes, std::atomic<uint64_t>&
 }
 
 template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shape& s, hipStream_t stream) {
+    constexpr int CHUNK_ROWS = chunk_rows<T>;
     Args a;
     a.d = *d;
     a.page_shift = __builtin_ctz(d->page_size);
@@ -834,12 +837,12 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
         const int prefix = 4 * (a.units + 1) * 4;
         const int64_t most = tiles * a.units * d->kv_heads;
         MMF_CHECK_ARG(most <= 0x3fffffff, "paged_attention: too many rows for one call");
-        const int cap = s.chunk ? 2048 : 512, grid = s.split || most > cap ? cap : (int)most;
+        const int cap = s.chunk ? 2048 * 128 / CHUNK_ROWS : 512, grid = s.split || most > cap ? cap : (int)most;
         if (s.chunk) {
             const int lds = chunk_lds<T, D> + prefix;
             static std::atomic<uint64_t> done{0};
             MMF_CHECK_ARG(!allow_lds(paged_attn_chunk_kernel<T, D>, chunk_lds<T, D> + PREFIX_MAX, done), "paged_attention: LDS");
-            hipLaunchKernelGGL((paged_attn_chunk_kernel<T, D>), dim3(grid), dim3(256), lds, stream, a);
+            hipLaunchKernelGGL((paged_attn_chunk_kernel<T, D>), dim3(grid), dim3(2 * CHUNK_ROWS), lds, stream, a);
         } else {
             const int lds = step_lds<T, D> + 16 + prefix;
             static std::atomic<uint64_t> done{0};
