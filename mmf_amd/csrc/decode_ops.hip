@@ -446,16 +446,20 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
             past[e] = d.history[at + w * d.length + k - w * cols];
         }
     }
+    const int l16 = tid & 15;
+    Segment first = {0.0, -INFINITY, 0};
+    if (tid >> 4 < W && l16 < segments) first = segs[(tid >> 4) * segments + l16];
     __syncthreads();
     for (int w0 = 0; w0 < W; w0 += 16) {                          // lse, by 16 lanes each: NaN marks a row without candidates
-        const int w = w0 + (tid >> 4), l16 = tid & 15;
+        const int w = w0 + (tid >> 4);
         const bool live = w < W && !done[w] && score[w] > NEG_INF;
-        float m = -INFINITY;
-        for (int s = live ? l16 : segments; s < segments; s += 16) m = fmaxf(m, segs[w * segments + s].top);
+        if (w0) first = live && l16 < segments ? segs[w * segments + l16] : Segment{0.0, -INFINITY, 0};
+        float m = live ? first.top : -INFINITY;
+        for (int s = live ? l16 + 16 : segments; s < segments; s += 16) m = fmaxf(m, segs[w * segments + s].top);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        double sum = 0.0;
-        for (int s = live ? l16 : segments; s < segments; s += 16) {
+        double sum = live && first.top > -INFINITY ? first.sum * (double)exp_down(first.top - m) : 0.0;
+        for (int s = live ? l16 + 16 : segments; s < segments; s += 16) {
             const Segment x = segs[w * segments + s];
             if (x.top > -INFINITY) sum += x.sum * (double)exp_down(x.top - m);
         }
@@ -571,25 +575,22 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     __syncthreads();
     if (!d.history) return;
     // through LDS, many columns at a time: in place as well
-#pragma unroll
-    for (int e = 0; e < KEEP; ++e)
-        if (tid + 256 * e < W * cols) cand_i[tid + 256 * e] = past[e];
-    __syncthreads();
     for (int64_t t0 = 0; t0 < d.length; t0 += cols) {
-        if (t0) {
-#pragma unroll 4
-            for (int k = tid; k < W * cols; k += 256) {
-                const int w = (int)(((float)k + 0.5f) * per_col);
-                const int64_t t = t0 + k - w * cols;
-                if (t < d.length) cand_i[k] = d.history[at + w * d.length + t];
+#pragma unroll
+        for (int e = 0; e < KEEP; ++e) {                              // these columns, and the next ones on their way
+            const int k = tid + 256 * e, w = (int)(((float)k + 0.5f) * per_col);
+            const int64_t t = t0 + cols + k - w * cols;
+            if (k < W * cols) {
+                cand_i[k] = past[e];
+                if (t < d.length) past[e] = d.history[at + w * d.length + t];
             }
-            __syncthreads();
         }
-#pragma unroll 4
-        for (int k = tid; k < W * cols; k += 256) {
-            const int w = (int)(((float)k + 0.5f) * per_col);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < KEEP; ++e) {
+            const int k = tid + 256 * e, w = (int)(((float)k + 0.5f) * per_col);
             const int64_t t = t0 + k - w * cols;
-            if (t < d.length) d.history_out[at + w * d.length + t] = t == d.step ? best_i[w] : cand_i[parent[w] * cols + k - w * cols];
+            if (k < W * cols && t < d.length) d.history_out[at + w * d.length + t] = t == d.step ? best_i[w] : cand_i[parent[w] * cols + k - w * cols];
         }
         __syncthreads();
     }

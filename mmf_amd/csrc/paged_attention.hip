@@ -7,7 +7,7 @@
 // scores (16 keys of every 32; lane ^ 32 the others), so maximum and sum need one exchange, and the probabilities are in the register order that the second
 // product O^T = V^T P^T takes (v_mfma_f32_32x32x16_bf16, or v_mfma_f32_32x32x2_f32 for the fp32 pool, whose operands are one row element per lane).
 //
-//   chunks (more than 32 rows per request and key head): a workgroup takes 128 rows, its four waves share the staged K and V tiles;
+//   chunks (more than 32 rows per request and key head): a workgroup takes 128 rows (fp32: 64), its waves share the staged K and V tiles;
 //   steps  (at most 32 rows):                           a workgroup takes all beams of a group that fit 32 rows, its four waves take different tiles.
 //
 // Keys are split over workgroups in runs of equal length for all requests, chosen on the device from the actual lengths (Plan below); runs are joined by a
@@ -24,7 +24,9 @@ typedef const __attribute__((address_space(1))) void* glb_vp;
 static __device__ uint4 g_zero16;
 
 constexpr int STEP_ROWS = 32;
-template <typename T> constexpr int chunk_rows = sizeof(T) == 2 ? 128 : 64;       // a wave per 32
+// Rows of a chunk's workgroup, a wave per 32.  fp32 is bound by its products and not by what it stages: fewer waves without rows at the end of a prompt count for more
+// (32 prompts of 70 .. 170 tokens, 12 heads of 64: 36.9 us with 128 rows, 35.6 with 64; bf16 reads every tile twice as often with 64).
+template <typename T> constexpr int chunk_rows = sizeof(T) == 2 ? 128 : 64;
 constexpr int UNITS_MAX = 960;         // requests (chunks) or groups of beams (steps) per launch
 constexpr int PREFIX_MAX = 4 * (UNITS_MAX + 1) * 4;
 
@@ -47,7 +49,7 @@ template <int RB> DEVI int at(int row, int chunk) { return row * RB + ((chunk ^ 
 // key0 + (l % ROWS).  NW waves share the tile, ROWS / NW rows in a row each.  Chunks, where these lie in one page (a tile starts on a page, or ROWS divide the page and
 // the tile's start): the wave reads them through a buffer descriptor that ends behind the last of them, and all that a lane adds to it is its place among them, the same
 // for every tile.  Otherwise every lane has an address of its own; in steps too, whose few tiles wait for the first bytes and not for the instructions before them (32
-// groups of 5 beams: 11.9 us, and 12.5 by descriptors; 270 GFLOP of chunks: 350 us, and STAGEUS by descriptors).
+// groups of 5 beams: 11.9 us, and 12.5 by descriptors; 270 GFLOP of chunks: 350 us, and 340 by descriptors).
 template <typename T, int D, int ROWS, int NW> struct Stager {
     static constexpr int RB = D * (int)sizeof(T), CPR = RB / 16, RPI = 64 / CPR, OWN = ROWS / NW, N = OWN / RPI;
     uint32_t offset[N];                // of a row's 16 bytes, in its page or among the wave's rows
