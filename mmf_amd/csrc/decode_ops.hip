@@ -8,27 +8,30 @@
 
 namespace {
 
-// inclusive sum over the workgroup; `total` gets the sum of all.  lds: one value per wave
-template <typename T> DEVI T block_scan(T v, int64_t* lds, T& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T s = v;
+// inclusive sum over the workgroup (up to 16 waves); `total` gets the sum of all.  lds: 16 values
+template <typename T> DEVI T wave_upto(T v, int lane) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const T t = __shfl_up(s, o, 64);
-        if (lane >= o) s += t;
+        const T t = __shfl_up(v, o, 64);
+        if (lane >= o) v += t;
     }
+    return v;
+}
+template <typename T> DEVI T block_scan(T v, int64_t* lds, T& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const T s = wave_upto(v, lane);
     __syncthreads();
     if (lane == 63) lds[wave] = s;
     __syncthreads();
-    T before = 0;
-    total = 0;
-#pragma unroll 1
-    for (int w = 0; w < (int)blockDim.x / 64; ++w) {
-        const T x = (T)lds[w];
-        if (w < wave) before += x;
-        total += x;
+    T x = lane < waves ? (T)lds[lane] : 0;
+    const T own = __shfl(x, wave, 64);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        const T t = __shfl_up(x, o, 64);
+        if (lane >= o) x += t;
     }
-    return s + before;
+    total = __shfl(x, 15, 64);
+    return s + __shfl(x, wave, 64) - own;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -47,54 +50,60 @@ constexpr int PLAN_THREADS = 1024;       // (256 where that is a thread per grou
 
 DEVI int blocks_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
-// Pages of released groups, back on the stack in the order of their rows and blocks; returns the new top.  A wave counts a row's pages, the counts are scanned,
-// a wave pushes them; `counts` holds one int per row, `list` another: the rows to release, in any order.
-DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, int* counts, int* list, int* released, int64_t* lds) {
+// Pages of released groups, back on the stack in the order of their rows and blocks; returns the new top.  As many rows at a time as there are threads: those to
+// release are listed, in any order; a wave counts the pages of a listed row, the counts are scanned over the rows, and a wave pushes them from there.
+struct Release { int blocks[PLAN_THREADS], place[PLAN_THREADS], list[PLAN_THREADS], listed; };
+DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, Release& x, int64_t* lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6, R = d.groups * d.beams;
-    for (int r = tid; r < R; r += blockDim.x) {
-        counts[r] = 0;
-        if (d.q_lens[r / d.beams] < 0) list[atomicAdd(released, 1)] = r;
-    }
-    __syncthreads();
-    const int n_list = *released;
 #pragma unroll 1
-    for (int k = wave; k < n_list; k += waves) {
-        int n = 0;
-        const int r = list[k], blocks = min(blocks_of(max(d.kv_lens[r / d.beams], 0), shift), d.blocks);
+    for (int r0 = 0; r0 < R; r0 += blockDim.x) {
+        const int g = min(r0 + tid, R - 1) / d.beams, q = d.q_lens[g], kv = d.kv_lens[g];
+        if (tid == 0) x.listed = 0;
+        __syncthreads();
+        x.place[tid] = 0;
+        if (r0 + tid < R && q < 0) {
+            x.blocks[tid] = min(blocks_of(max(kv, 0), shift), d.blocks);
+            x.list[atomicAdd(&x.listed, 1)] = tid;
+        }
+        __syncthreads();
+        const int listed = x.listed;
+#pragma unroll 2
+        for (int k = wave; k < listed; k += waves) {
+            const int r = x.list[k], blocks = x.blocks[r];
+            const int* owned = d.owned + (size_t)(r0 + r) * d.blocks;
+            int n = 0;
 #pragma unroll 4
-        for (int j = lane; j < blocks; j += 64) n += d.owned[(size_t)r * d.blocks + j] >= 0;
+            for (int j = lane; j < blocks; j += 64) n += owned[j] >= 0;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-        if (lane == 0) counts[r] = n;
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (int r0 = 0; r0 < R; r0 += blockDim.x) {                  // counts[r] becomes the row's place on the stack
-        const int r = r0 + tid, n = r < R ? counts[r] : 0;
+            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+            if (lane == 0) x.place[r] = n;
+        }
+        __syncthreads();
+        const int n = x.place[tid];
         int total;
         const int upto = block_scan(n, lds, total);
-        if (r < R) counts[r] = n ? top + upto - n : -1;
-        top = min(top + total, d.free_capacity);
-    }
-    __syncthreads();
+        x.place[tid] = top + upto - n;
+        __syncthreads();
 #pragma unroll 1
-    for (int k = wave; k < n_list; k += waves) {
-        const int r = list[k];
-        int at = counts[r];
-        if (at < 0) continue;
-        const int blocks = min(blocks_of(max(d.kv_lens[r / d.beams], 0), shift), d.blocks);
-        for (int j0 = 0; j0 < blocks; j0 += 64) {
-            const int p = j0 + lane < blocks ? d.owned[(size_t)r * d.blocks + j0 + lane] : -1;
-            const uint64_t m = __ballot(p >= 0);
-            const int to = at + __popcll(m & ((1ull << lane) - 1));
-            if (p >= 0) {
-                if (to < d.free_capacity) d.free_pages[to] = p;
-                else flag_page_error();                          // more pages came back than the pool has: one was given back twice
+        for (int k = wave; k < listed; k += waves) {
+            const int r = x.list[k], blocks = x.blocks[r];
+            const int* owned = d.owned + (size_t)(r0 + r) * d.blocks;
+            int at = x.place[r];
+#pragma unroll 1
+            for (int j0 = 0; j0 < blocks; j0 += 64) {
+                const int p = j0 + lane < blocks ? owned[j0 + lane] : -1;
+                const uint64_t m = __ballot(p >= 0);
+                const int to = at + __popcll(m & ((1ull << lane) - 1));
+                if (p >= 0) {
+                    if (to < d.free_capacity) d.free_pages[to] = p;
+                    else flag_page_error();                      // more pages came back than the pool has: one was given back twice
+                }
+                at += __popcll(m);
             }
-            at += __popcll(m);
         }
+        top = min(top + total, d.free_capacity);
+        __syncthreads();
     }
-    __syncthreads();
     return top;
 }
 
@@ -136,18 +145,20 @@ DEVI void plan_row(const mmf_paged_plan_desc& d, int shift, const PlanGroup& g, 
 // rows_too: a row by one thread, or by eight where some have more than four tokens; else the second launch takes workgroups for each
 __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc d, int shift, int rows_too) {
     __shared__ int64_t lds[PLAN_THREADS / 64];
-    __shared__ int taken, refused, flags, released;               // flags: 1 a group is released, 2 a row has many tokens
+    __shared__ int taken, refused, flags;                         // flags: 1 a group is released, 2 a row has many tokens
+    __shared__ Release release;
     const int tid = threadIdx.x, threads = blockDim.x, W = d.beams, per = d.shared ? 1 : W;
     PlanGroup* ws = reinterpret_cast<PlanGroup*>(d.ws);
-    int* tail = reinterpret_cast<int*>(ws + d.groups);             // [0]: the top the pages are taken from, [4 ..]: plan_release's counts and list
-    if (tid == 0) { taken = 0; refused = 0; flags = 0; released = 0; }
+    int* tail = reinterpret_cast<int*>(ws + d.groups);             // [0]: the top the pages are taken from
+    if (tid == 0) { taken = 0; refused = 0; flags = 0; }
+    const int g_first = min(tid, d.groups - 1), q_first = d.q_lens[g_first], kv_first = d.kv_lens[g_first];
     for (int i = tid; i < 3 * d.groups * W; i += threads) d.copies[i] = -1;
     const int told = d.free_top[0];
     int top = min(max(told, 0), d.free_capacity);
     if (tid == 0 && top != told) flag_page_error();
     __syncthreads();
-    int most = 0, least = 0;
-    for (int g = tid; g < d.groups; g += threads) {
+    int most = max(q_first, 0), least = min(q_first, 0);
+    for (int g = tid + threads; g < d.groups; g += threads) {
         const int q = d.q_lens[g];
         most = max(most, q);
         least = min(least, q);
@@ -155,7 +166,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc 
     const int f = (least < 0) | (most > 4) << 1;
     if (f) atomicOr(&flags, f);
     __syncthreads();
-    if (flags & 1) top = plan_release(d, shift, top, tail + 4, tail + 4 + d.groups * W, &released, lds);
+    if (flags & 1) top = plan_release(d, shift, top, release, lds);
     const int per_row = flags & 2 ? 8 : 1;
     int carry_need = 0, total;
     int64_t carry_rows = 0, total64;
@@ -163,7 +174,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc 
     for (int g0 = 0; g0 < d.groups; g0 += threads) {
         const int g = g0 + tid;
         const bool in = g < d.groups;
-        const int q = in ? d.q_lens[g] : 0, kv = in ? max(d.kv_lens[g], 0) : 0, n = max(q, 0);
+        const int q = !in ? 0 : g0 ? d.q_lens[g] : q_first, kv = !in ? 0 : max(g0 ? d.kv_lens[g] : kv_first, 0), n = max(q, 0);
         const int64_t rows = (int64_t)per * n, start = carry_rows + block_scan(rows, lds, total64) - rows;
         carry_rows += total64;
         const bool fits = (int64_t)kv + n <= (int64_t)d.blocks << shift && start + rows <= d.rows;
@@ -696,7 +707,7 @@ int mmf_decode_take_error(void) {
 }
 
 int64_t mmf_paged_plan_ws_bytes(int groups, int beams) {
-    return groups > 0 && beams > 0 ? (int64_t)groups * (int64_t)sizeof(PlanGroup) + 16 + 8 * (int64_t)groups * beams : 0;
+    return groups > 0 && beams > 0 ? (int64_t)groups * (int64_t)sizeof(PlanGroup) + 16 : 0;
 }
 
 int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream) {
