@@ -121,19 +121,26 @@ Plan plan_pages(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& table
     const Tensor none;
     auto o = [&](size_t i) -> const Tensor* { return out.empty() ? &none : &out[i]; };
     On on({&q_lens, &kv_lens, &tables, &owned, &free_pages, &free_top, o(0), o(1), o(2), o(3), o(4), o(5), o(6), o(7)});
+    const int64_t ws_bytes = mmf_paged_plan_ws_bytes((int)G, (int)beams);
+    void* ws;                                                     // (small: next to the results it costs no allocation of its own)
+    Tensor ws_owner;
     if (out.empty()) {
-        Carver c(Carver::room(8 * rows) + Carver::room(4 * n) + 2 * Carver::room(4 * G) + Carver::room(4 * rows) + Carver::room(12 * R) + 32, q_lens);
+        Carver c(Carver::room(ws_bytes) + Carver::room(8 * rows) + Carver::room(4 * n) + 2 * Carver::room(4 * G) + Carver::room(4 * rows) + Carver::room(12 * R) + 32, q_lens);
+        ws = c.base.data_ptr();
+        c.at = Carver::room(ws_bytes);
         const Tensor slots = c.take({rows}, at::kLong), start = c.take({n}, at::kInt), granted = c.take({G}, at::kInt), kv = c.take({G}, at::kInt),
                      pos = c.take({rows}, at::kInt), copies = c.take({R, 3}, at::kInt), top = c.take({1}, at::kInt), refused = c.take({1}, at::kInt);
         p = {start, granted, kv, slots, pos, copies, top, refused};
+    } else {
+        ws_owner = workspace(ws_bytes, q_lens);
+        ws = P(ws_owner);
     }
-    const Tensor ws = workspace(mmf_paged_plan_ws_bytes((int)G, (int)beams), q_lens);
     mmf_paged_plan_desc d = {};
     d.q_lens = PT<int32_t>(q_lens); d.kv_lens = PT<int32_t>(kv_lens); d.tables = PT<int32_t>(tables); d.owned = PT<int32_t>(owned);
     d.free_pages = PT<int32_t>(free_pages); d.free_top = PT<int32_t>(free_top);
     d.q_start = PT<int32_t>(std::get<0>(p)); d.granted = PT<int32_t>(std::get<1>(p)); d.kv_out = PT<int32_t>(std::get<2>(p)); d.slots = PT<int64_t>(std::get<3>(p));
     d.positions = PT<int32_t>(std::get<4>(p)); d.copies = PT<int32_t>(std::get<5>(p)); d.top_out = PT<int32_t>(std::get<6>(p)); d.refused = PT<int32_t>(std::get<7>(p));
-    d.ws = P(ws);
+    d.ws = ws;
     d.groups = (int)G; d.beams = (int)beams; d.blocks = (int)tables.size(1); d.page_size = (int)page_size; d.rows = (int)rows; d.shared = shared;
     d.free_capacity = (int)free_pages.numel();
     done(mmf_paged_plan(&d, on.stream), "mmf_paged_plan");
