@@ -37,7 +37,8 @@ template <typename T> DEVI T block_scan(T v, int64_t* lds, T& total) {
 // ------------------------------------------------------------------------------------------------
 // the plan of a step.  Whole numbers only; a few bytes per request and 12 per new token: latency is all there is to it.  One workgroup takes back the pages of
 // finished groups and scans the groups (a thread each: what a group needs, what those before it took); the rows' tokens and blocks are filled in by the
-// same launch where they are few, and by a second one over the whole chip where not.
+// same launch where they are few, and by a second one over the whole chip where not.  32 groups of 5 beams with a token each: 4.3 us;
+// 512 requests, 51 of them released, with 136 thousand new tokens: 14.8 us (four dependent trips to memory, two for the released pages, and three scans) and 4.2 for the rows.
 // ------------------------------------------------------------------------------------------------
 struct PlanGroup {      // what the scan leaves for the rows of a group
     int base;           // pages taken by the groups before it
@@ -47,6 +48,7 @@ struct PlanGroup {      // what the scan leaves for the rows of a group
 };
 
 constexpr int PLAN_THREADS = 1024;       // (256 where that is a thread per group)
+constexpr int PLAN_MANY = 128;           // tokens from which a row is walked by the whole workgroup
 
 DEVI int blocks_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
@@ -142,7 +144,7 @@ DEVI void plan_row(const mmf_paged_plan_desc& d, int shift, const PlanGroup& g, 
     }
 }
 
-// rows_too: a row by one thread, or by eight where some have more than four tokens; else the second launch takes workgroups for each
+// rows_too: a row by one thread, by eight where some have more than four tokens, by all where it has many; else the second launch takes workgroups for each
 __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc d, int shift, int rows_too) {
     __shared__ int64_t lds[PLAN_THREADS / 64];
     __shared__ int taken, refused, flags;                         // flags: 1 a group is released, 2 a row has many tokens
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc 
         most = max(most, q);
         least = min(least, q);
     }
-    const int f = (least < 0) | (most > 4) << 1;
+    const int f = (least < 0) | (most > 4) << 1 | (most > PLAN_MANY) << 2;
     if (f) atomicOr(&flags, f);
     __syncthreads();
     if (flags & 1) top = plan_release(d, shift, top, release, lds);
@@ -207,10 +209,22 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(mmf_paged_plan_desc 
         tail[0] = top;
     }
     if (!rows_too) return;
+    if (tid == 0) release.listed = 0;
+    __syncthreads();
 #pragma unroll 1
     for (int r = tid / per_row; r < d.groups * W; r += threads / per_row) {
         const int g = r / W;
-        plan_row(d, shift, ws[g], r, r - g * W, d.shared ? d.q_start[g] : d.q_start[r], top, tid % per_row, per_row);
+        const PlanGroup x = ws[g];
+        if ((flags & 4) && x.granted > PLAN_MANY) {
+            if (tid % per_row == 0) release.list[atomicAdd(&release.listed, 1)] = r;
+        } else plan_row(d, shift, x, r, r - g * W, d.shared ? d.q_start[g] : d.q_start[r], top, tid % per_row, per_row);
+    }
+    if (!(flags & 4)) return;
+    __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < release.listed; ++k) {
+        const int r = release.list[k], g = r / W;
+        plan_row(d, shift, ws[g], r, r - g * W, d.shared ? d.q_start[g] : d.q_start[r], top, tid, threads);
     }
 }
 __global__ __launch_bounds__(256) void plan_rows_kernel(mmf_paged_plan_desc d, int shift) {
@@ -221,8 +235,9 @@ __global__ __launch_bounds__(256) void plan_rows_kernel(mmf_paged_plan_desc d, i
 }
 
 // ------------------------------------------------------------------------------------------------
-// new keys and values into their slots.  Every byte moves once each way; a thread moves one VT (16 bytes, or one element
-// where a row does not start on 16 bytes).
+// new keys and values into their slots.  Every byte moves once each way, and memory bounds it: 16384 rows of 8 heads of 128 in bf16, 27 us for 121 MB; 160 rows of 12 heads
+// of 64: 2.3 us, an empty launch.  A thread moves one VT: 16 bytes, or one element where a row does not start on 16 bytes (134 MB that caches hold: 22 us by 16 bytes,
+// 122 by elements).
 // ------------------------------------------------------------------------------------------------
 template <typename VT>
 __global__ __launch_bounds__(256) void paged_write_kernel(mmf_paged_write_desc d, int esize, int per_token) {
@@ -253,6 +268,10 @@ __global__ __launch_bounds__(256) void paged_write_kernel(mmf_paged_write_desc d
 // Within a row the order is the logits' own, so a first kernel takes every row in segments, a workgroup each with the segment in its registers, and leaves the segment's
 // maximum, its sum of exponentials and its W largest; a second one merges the segments and beams of a group.  Both pick W out of N in the same way: of the maxima of
 // 64 groups of threads the W-th largest is a bar that at least W values reach, and few more do; those are ranked by counting.
+//
+// 128 rows of 128000 logits in bf16, 8 beams: 15 us for the rows (33 MB; half of it arithmetic, 16 instructions a logit of which the exponential and its correction are 7,
+// that starts when most loads have landed) and 10 for the merge; 160 rows of 5050 in fp32, 5 beams: 6.3 and 6.9 us.  The merge is a chain of trips to memory and to
+// LDS by a workgroup per group: what does not wait for the sums (lists, segments, the history's first columns) is read first.
 // ------------------------------------------------------------------------------------------------
 constexpr double NEG_INF = -__builtin_huge_val();
 constexpr int CHUNKS = 4, LIST = 1024, KEEP = LIST / 256;                            // 16-byte pieces of a segment per thread
@@ -607,7 +626,8 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     }
 }
 
-// Segments of a row: as long as a workgroup holds, and shorter where few rows would leave compute units idle (four workgroups for each), down to a piece per thread
+// Segments of a row: as long as a workgroup holds, and shorter where few rows would leave compute units idle (four workgroups for each; with two or eight the two sizes
+// above take the same within 2 %), down to a piece per thread
 int beam_segments(int rows, int64_t vocab, bool f32, int* length) {
     const int64_t least = (vocab + (f32 ? seg_max<float> : seg_max<bf16>) - 1) / (f32 ? seg_max<float> : seg_max<bf16>), fill = (1024 + rows - 1) / rows;
     const int64_t most = vocab / (f32 ? 1024 : 2048);
@@ -622,6 +642,8 @@ int beam_segments(int rows, int64_t vocab, bool f32, int* length) {
 // block tables after a selection.  A block that is full is only read from here on: the children share it.  The block that goes on being
 // written has to be each beam's own: the first child of a beam keeps its page, the other children take the pages of the beams that have
 // no child, of which there are exactly as many, and get its tokens copied.  A page that is copied from is never copied to.
+// The tables are a workgroup per group; the copies a launch over rows and planes that leaves at once where there is nothing to copy.  32 groups of 5 beams, 8 planes of
+// 12 heads of 64, half a page of 16 to copy: 8.7 us for 12.5 MB, two launches and their trips to memory; 8 groups of 8 beams, 32 planes of 8 heads of 128, 68 MB: 21 us.
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void reorder_tables_kernel(mmf_paged_reorder_desc d) {
     __shared__ int pages[LIST], copied[MMF_BEAMS_MAX];
@@ -669,7 +691,8 @@ __global__ __launch_bounds__(256) void reorder_tables_kernel(mmf_paged_reorder_d
     if ((part < 0 || part >= d.blocks) && tid < 3 * W) d.copies[3 * (size_t)g * W + tid] = -1;
 }
 
-// the first copies[r][2] tokens of page copies[r][0] to page copies[r][1], in every plane (keys and values of every layer)
+// the first copies[r][2] tokens of page copies[r][0] to page copies[r][1], in every plane (keys and values of every layer).  VT: 16 bytes, or an element where rows
+// do not start on 16 (64 pages of 8 heads of 17 tokens in 32 planes: 20 us with 128 columns, 32 with 125)
 template <typename VT>
 __global__ __launch_bounds__(256) void copy_pages_kernel(mmf_paged_copy_desc d, int esize) {
     const int r = blockIdx.x;
@@ -717,9 +740,11 @@ int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream) {
     MMF_CHECK_ARG(d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->groups <= 0x0fffffff / d->beams, "paged_plan: 1 .. 32 beams");
     MMF_CHECK_ARG(d->page_size >= 1 && d->page_size <= MMF_PAGE_MAX && (d->page_size & (d->page_size - 1)) == 0, "paged_plan: page_size is a power of two up to 1024");
     MMF_CHECK_ARG((int64_t)d->blocks * d->page_size <= 0x40000000 && d->rows <= 0x40000000, "paged_plan: more than 2^30 tokens");
-    // one workgroup walks up to a thousand tokens, or a few for each of as many rows as it has threads; more is work for the whole chip and a second launch
+    // One workgroup walks up to a thousand tokens, or a few for each of as many rows as it has threads; more is work for the whole chip and a second launch.  32 groups of 5
+    // beams, a token each: 4.3 us in one launch, 6.0 in two; 512 prompts of up to 2048 tokens: 306 us in one, 18.5 in two.
     const int64_t rows = (int64_t)d->groups * d->beams;
-    const bool one = d->rows <= 1024 || (d->rows <= 4 * rows && rows <= 4 * PLAN_THREADS);
+    const int64_t walked = (int64_t)d->rows * (d->shared ? d->beams : 1);      // (every row of a shared group fills its table; rows of many tokens: fewer than a thread each)
+    const bool one = walked <= 1024 || (walked <= 4 * rows && rows <= 4 * PLAN_THREADS);
     const int shift = __builtin_ctz(d->page_size);
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(rows <= 256 ? 256 : PLAN_THREADS), 0, (hipStream_t)stream, *d, shift, (int)one);
     MMF_CHECK_LAUNCH();

@@ -12,6 +12,15 @@
 //
 // Keys are split over workgroups in runs of equal length for all requests, chosen on the device from the actual lengths (Plan below); runs are joined by a
 // second kernel, launched only where a request can be split at all.
+//
+// What bounds it, and what it measured (MI355X; a copy of 1 GiB reaches 5.18 TB/s, a bf16 product of 8192^3 1262 TFLOP/s, an fp32 one of 4096^3 139):
+//   long caches   8 requests of 16384 .. 65536 keys, 32 heads on 8, head_dim 128, one token: 191 us, 5.3 TB/s of pages.  Memory.
+//   steps         32 groups of 5 beams, 120 .. 181 keys of which the prompt's pages are shared, 12 heads of 64: 11.9 us for 21.5 MB.  The chain lengths, table,
+//                 first tile, four tiles, meeting of the waves; with every beam reading the shared pages itself 25.3 us.
+//   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 336 us, 803 TFLOP/s.  Products (512 cycles per 32 keys of a wave) and vector instructions (500) of
+//                 the two waves that a compute unit's SIMD holds; without exponentials, or without reading the operands, it takes 320 and 328 us.
+//   fp32 prompts  32 prompts of 70 .. 170 tokens, 12 heads of 64: 35.6 us.  The products of the longest prompts (3.5 us per 32 keys for two waves on a SIMD) behind 10 us
+//                 of lengths, plan, queries, first tile and output.
 #include "common.h"
 #include "mmf_amd.h"
 #include "paged_common.h"
@@ -785,6 +794,10 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(Args a) {
     }
 }
 
+// Which kernel, and how keys are split.  Up to 32 rows per key head go through the step kernel, whose waves take different keys; more have rows enough for a wave each.
+// Workgroups to aim at when keys are split: 512 steps (two on every compute unit; long caches: 191 us, with 256 190, with 1024 199), 768 chunks of 128 rows (with 512
+// 340 us as well, with 1024 347: longest first, the short last runs fill the gaps).  Shortest run 512 keys: one request of 500 keys takes 8.2 us in one piece and 14.9 split
+// by 256, 4 requests of 1000 keys 19.9 and 17.7; 2 chunks of 64 tokens over 4000 keys take 37.4 us, 43.8 with runs of 1024 and 45.5 with runs of 256.
 struct Shape { bool chunk, split; int nb, target, run_min, parts; int64_t ws; };
 Shape shape_of(const mmf_paged_attn_desc* d) {
     Shape s;
@@ -793,7 +806,7 @@ Shape shape_of(const mmf_paged_attn_desc* d) {
     s.nb = s.chunk ? 1 : (int)(STEP_ROWS / rows < d->beams ? STEP_ROWS / rows : d->beams);
     const int tile = !s.chunk ? STEP_ROWS : d->is_f32 ? chunk_rows<float> : chunk_rows<bf16>;
     s.target = s.chunk ? 768 * 128 / tile : 512;
-    s.run_min = s.chunk ? 1024 : 256;
+    s.run_min = 512;
     s.parts = s.chunk ? 2 * s.target : 1024;
     s.split = (int64_t)d->blocks * d->page_size > s.run_min;
     s.ws = s.split ? (int64_t)s.parts * tile * (d->head_dim + 2) * 4 : 0;

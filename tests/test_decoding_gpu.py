@@ -47,7 +47,8 @@ def plan_both(q_lens, kv_lens, tables, owned, free, top, page, rows, beams, shar
     return want, tables, owned, free
 
 
-@pytest.mark.parametrize("page,beams,shared,groups", [(1, 1, False, 1), (16, 1, True, 7), (16, 5, False, 9), (16, 5, True, 9), (8, 32, False, 3), (64, 2, True, 1500), (1024, 3, False, 40),
+@pytest.mark.parametrize("page,beams,shared,groups", [(1, 1, False, 1), (16, 1, True, 7), (16, 5, False, 9), (16, 5, True, 9), (8, 32, False, 3), (64, 2, True, 1500), (1024, 3, False, 40), (64, 1, True, 2), (64, 5, True, 2), (64, 2, False, 2),
+                                                      (64, 32, True, 100),
                                                       (32, 1, False, 2100)])
 def test_plan_grows_releases_and_waits_like_the_plain_form(page, beams, shared, groups):
     """Five steps of one pool: prompts, single tokens, chunks, finished groups, more tokens than pages, tables or rows hold."""
