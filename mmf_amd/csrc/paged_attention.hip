@@ -18,7 +18,7 @@
 //   steps         32 groups of 5 beams, 120 .. 181 keys of which the prompt's pages are shared, 12 heads of 64: 11.9 us for 21.5 MB.  The chain lengths, table,
 //                 first tile, four tiles, meeting of the waves; with every beam reading the shared pages itself 25.3 us.
 //   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 336 us, 803 TFLOP/s.  Products (512 cycles per 32 keys of a wave) and vector instructions (500) of
-//                 the two waves that a compute unit's SIMD holds; without exponentials, or without reading the operands, it takes 320 and 328 us.
+//                 the two waves that a SIMD holds; without exponentials it takes 320 us, without staging 293, without barriers too 280.
 //   fp32 prompts  32 prompts of 70 .. 170 tokens, 12 heads of 64: 35.6 us.  The products of the longest prompts (3.5 us per 32 keys for two waves on a SIMD) behind 10 us
 //                 of lengths, plan, queries, first tile and output.
 #include "common.h"
