@@ -278,6 +278,33 @@ def test_max_q_larger_than_any_request_and_out_in_place_of_q(dtype):
     assert torch.equal(out[:29], a[:29])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page", [4, 16, 64])
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_outside_the_pool_read_as_zeros(dtype, page, new):
+    from mmf_amd import _native as nat
+    c = attend_case([150, 90], [new, new], heads=4, kv_heads=2, page=page, dtype=dtype)
+    empty = torch.cat([torch.zeros_like(c["key_cache"][:1]), c["key_cache"]]), torch.cat([torch.zeros_like(c["value_cache"][:1]), c["value_cache"]])
+    want_t, t = c["tables"] + 1, c["tables"] + 1
+    for block in (0, 40 // page, 149 // page):
+        want_t[0, block] = 0
+    rest = dict(kv_lens=c["kv_lens"], q_start=c["q_start"], q_lens=c["q_lens"], max_q=new)
+    want = D().attend_pages(c["q"], *empty, want_t, **rest)
+    for bad in (-1, -2 ** 31, empty[0].shape[0], 2 ** 31 - 1):
+        for block in (0, 40 // page, 149 // page):
+            t[0, block] = bad
+        nat.take_index_error()
+        got = D().attend_pages(c["q"], *empty, t, **rest)
+        assert nat.take_index_error()
+        assert torch.equal(got[:2 * new], want[:2 * new])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_query_heads_on_a_key_head_than_a_step_has_rows(dtype):
+    attend_check(attend_case([70, 1, 33], [1, 1, 1], heads=64, kv_heads=1, dim=64, dtype=dtype))
+    attend_check(attend_case([70, 40], [3, 2], heads=66, kv_heads=2, dim=128, dtype=dtype))
+
+
 def test_pages_outside_the_pool_are_reported_and_other_requests_do_not_notice():
     from mmf_amd import _native as nat
     for new, dtype in ((1, torch.bfloat16), (40, torch.bfloat16), (1, torch.float32), (40, torch.float32)):
