@@ -38,7 +38,7 @@ template <typename T> DEVI T block_scan(T v, int64_t* lds, T& total) {
 // the plan of a step.  Whole numbers only; a few bytes per request and 12 per new token: latency is all there is to it.  One workgroup takes back the pages of
 // finished groups and scans the groups (a thread each: what a group needs, what those before it took); the rows' tokens and blocks are filled in by the
 // same launch where they are few, and by a second one over the whole chip where not.  32 groups of 5 beams with a token each: 4.3 us;
-// 512 requests, 51 of them released, with 136 thousand new tokens: 14.8 us (four dependent trips to memory, two for the released pages, and three scans) and 4.2 for the rows.
+// 512 requests, 51 of them released, with 136 thousand new tokens: 13.6 us (four dependent trips to memory, two for the released pages, and three scans) and 4.3 for the rows.
 // ------------------------------------------------------------------------------------------------
 struct PlanGroup {      // what the scan leaves for the rows of a group
     int base;           // pages taken by the groups before it
@@ -53,10 +53,10 @@ constexpr int PLAN_MANY = 128;           // tokens from which a row is walked by
 DEVI int blocks_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
 // Pages of released groups, back on the stack in the order of their rows and blocks; returns the new top.  As many rows at a time as there are threads: those to
-// release are listed, in any order; a wave counts the pages of a listed row, the counts are scanned over the rows, and a wave pushes them from there.
+// release are listed, in any order; 16 lanes count the pages of a listed row, the counts are scanned over the rows, and 16 lanes push them from there.
 struct Release { int blocks[PLAN_THREADS], place[PLAN_THREADS], list[PLAN_THREADS], listed; };
 DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, Release& x, int64_t* lds) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6, R = d.groups * d.beams;
+    const int tid = threadIdx.x, l16 = tid & 15, team = tid >> 4, teams = blockDim.x >> 4, R = d.groups * d.beams;
 #pragma unroll 1
     for (int r0 = 0; r0 < R; r0 += blockDim.x) {
         const int g = min(r0 + tid, R - 1) / d.beams, q = d.q_lens[g], kv = d.kv_lens[g];
@@ -69,16 +69,16 @@ DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, Release&
         }
         __syncthreads();
         const int listed = x.listed;
-#pragma unroll 2
-        for (int k = wave; k < listed; k += waves) {
+#pragma unroll 1
+        for (int k = team; k < listed; k += teams) {
             const int r = x.list[k], blocks = x.blocks[r];
             const int* owned = d.owned + (size_t)(r0 + r) * d.blocks;
             int n = 0;
-#pragma unroll 4
-            for (int j = lane; j < blocks; j += 64) n += owned[j] >= 0;
+#pragma unroll 8
+            for (int j = l16; j < blocks; j += 16) n += owned[j] >= 0;
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-            if (lane == 0) x.place[r] = n;
+            for (int o = 8; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+            if (l16 == 0) x.place[r] = n;
         }
         __syncthreads();
         const int n = x.place[tid];
@@ -87,20 +87,24 @@ DEVI int plan_release(const mmf_paged_plan_desc& d, int shift, int top, Release&
         x.place[tid] = top + upto - n;
         __syncthreads();
 #pragma unroll 1
-        for (int k = wave; k < listed; k += waves) {
+        for (int k = team; k < listed; k += teams) {
             const int r = x.list[k], blocks = x.blocks[r];
             const int* owned = d.owned + (size_t)(r0 + r) * d.blocks;
             int at = x.place[r];
-#pragma unroll 1
             for (int j0 = 0; j0 < blocks; j0 += 64) {
-                const int p = j0 + lane < blocks ? owned[j0 + lane] : -1;
-                const uint64_t m = __ballot(p >= 0);
-                const int to = at + __popcll(m & ((1ull << lane) - 1));
-                if (p >= 0) {
-                    if (to < d.free_capacity) d.free_pages[to] = p;
-                    else flag_page_error();                      // more pages came back than the pool has: one was given back twice
+                int p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = j0 + 16 * e + l16 < blocks ? owned[j0 + 16 * e + l16] : -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t m = (uint32_t)(__ballot(p[e] >= 0) >> (tid & 48)) & 0xffff;
+                    const int to = at + __popc(m & ((1u << l16) - 1));
+                    if (p[e] >= 0) {
+                        if (to < d.free_capacity) d.free_pages[to] = p[e];
+                        else flag_page_error();                  // more pages came back than the pool has: one was given back twice
+                    }
+                    at += __popc(m);
                 }
-                at += __popcll(m);
             }
         }
         top = min(top + total, d.free_capacity);
@@ -741,7 +745,7 @@ int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream) {
     MMF_CHECK_ARG(d->page_size >= 1 && d->page_size <= MMF_PAGE_MAX && (d->page_size & (d->page_size - 1)) == 0, "paged_plan: page_size is a power of two up to 1024");
     MMF_CHECK_ARG((int64_t)d->blocks * d->page_size <= 0x40000000 && d->rows <= 0x40000000, "paged_plan: more than 2^30 tokens");
     // One workgroup walks up to a thousand tokens, or a few for each of as many rows as it has threads; more is work for the whole chip and a second launch.  32 groups of 5
-    // beams, a token each: 4.3 us in one launch, 6.0 in two; 512 prompts of up to 2048 tokens: 306 us in one, 18.5 in two.
+    // beams, a token each: 4.3 us in one launch, 6.0 in two; 512 prompts of up to 2048 tokens: 306 us in one, 17.4 in two.
     const int64_t rows = (int64_t)d->groups * d->beams;
     const int64_t walked = (int64_t)d->rows * (d->shared ? d->beams : 1);      // (every row of a shared group fills its table; rows of many tokens: fewer than a thread each)
     const bool one = walked <= 1024 || (walked <= 4 * rows && rows <= 4 * PLAN_THREADS);

@@ -52,7 +52,7 @@ def _lib():
 def plan_pages(q_lens, kv_lens, tables, owned, free_pages, free_top, *, page_size, rows, beams=1, shared=False, out=None):
     """Pages and slots of a step, from lengths on the device.
 
-    q_lens int32 [groups]: new tokens of each row of a group (`shared`: of the group, all of whose rows see them, as a prompt); negative: the group is done, the
+    q_lens int32 [groups]: new tokens of each row of a group (`shared`: of the group, while its rows still have one table: all see them, as a prompt); negative: the group is done, the
     pages its rows own go back on the free list and its length becomes 0.  kv_lens int32 [groups]: tokens in the cache.  tables, owned int32 [groups * beams,
     blocks]: the block tables, and which page each row took itself (both written in place).  free_pages int32 [capacity], free_top int32 [1]: the free list, pages
     are taken from its top.  rows: rows of the step's token buffers; the tokens of a group (of each of its beams) follow those of the group before.
