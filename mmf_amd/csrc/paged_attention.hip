@@ -17,7 +17,7 @@
 //   long caches   8 requests of 16384 .. 65536 keys, 32 heads on 8, head_dim 128, one token: 191 us, 5.3 TB/s of pages.  Memory.
 //   steps         32 groups of 5 beams, 120 .. 181 keys of which the prompt's pages are shared, 12 heads of 64: 11.9 us for 21.5 MB.  The chain lengths, table,
 //                 first tile, four tiles, meeting of the waves; with every beam reading the shared pages itself 25.3 us.
-//   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 336 us, 803 TFLOP/s.  Products (512 cycles per 32 keys of a wave) and vector instructions (500) of
+//   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 333 us, 810 TFLOP/s.  Products (512 cycles per 32 keys of a wave) and vector instructions (500) of
 //                 the two waves that a SIMD holds; without exponentials it takes 320 us, without staging 293, without barriers too 280.
 //   fp32 prompts  32 prompts of 70 .. 170 tokens, 12 heads of 64: 35.6 us.  The products of the longest prompts (3.5 us per 32 keys for two waves on a SIMD) behind 10 us
 //                 of lengths, plan, queries, first tile and output.
@@ -358,6 +358,7 @@ DEVI Unit unit_of(const Args& a, int u) {
 }
 
 struct Plan {
+    bool split;
     int run, items, parts, joins;
     int* order;      // [units] the units, longest first (up to 64 of them: else as they come)
     int* item0;      // [units + 1] first item of each unit, in that order
@@ -386,13 +387,24 @@ DEVI int wave_sum_int(int v) {
     return v;
 }
 
-// `lds`: 4 (units + 1) ints; every wave ends with the same plan (the first one writes it).  Where nothing can be split (all lengths within the shortest run) there is
-// no run to choose, and steps have nothing to plan: item = (unit, head).
-template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
+// Whether there is anything to split: tables may have room for long requests (a.split) that are not there.  32 requests of 150 keys, 12 heads of 64, in tables for 4096:
+// 9.6 us with this look at the lengths, 17.7 without it, 7.8 in tables for 512.
+DEVI bool any_long(const Args& a) {
+    if (!a.split) return false;
+    int most = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x & 63; i < a.d.requests / a.d.beams; i += 64) most = max(most, a.d.kv_lens[i]);
+    return __ballot(most > a.run_min) != 0;
+}
+
+// `lds`: 4 (units + 1) ints; every wave ends with the same plan (the first one writes it).  Where nothing is split there is no run to choose, and steps have nothing to
+// plan: item = (unit, head).
+template <int TILE> DEVI Plan make_plan(const Args& a, bool split_any, int* lds) {
     const int lane = threadIdx.x & 63;
     Plan p;
     p.run = 0x3fffffff;
-    if (!a.split && TILE == STEP_ROWS) {
+    p.split = split_any;
+    if (!split_any && TILE == STEP_ROWS) {
         p.items = a.units * a.d.kv_heads;
         return p;
     }
@@ -400,9 +412,10 @@ template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     p.part0 = lds + a.units + 1;
     p.join0 = lds + 2 * (a.units + 1);
     p.order = lds + 3 * (a.units + 1);
+    const Unit first = unit_of(a, min(lane, a.units - 1));                    // (64 units at most, as a rule: looked up once)
     int64_t work = 0;
-    for (int u = a.split ? lane : a.units; u < a.units; u += 64) {
-        const Unit x = unit_of(a, u);
+    for (int u = split_any ? lane : a.units; u < a.units; u += 64) {
+        const Unit x = u < 64 ? first : unit_of(a, u);
         work += (int64_t)tiles_of<TILE>(a, x) * x.kv;
     }
     work = wave_add(work) * a.d.kv_heads;
@@ -410,11 +423,11 @@ template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     // Steps: each request's last run is a short one; lengthen the runs until the workgroups that are resident together hold all of them.
     // Either: lengthen them until the partial results have room.
 #pragma unroll 1
-    for (int round = 0; a.split; ++round) {
+    for (int round = 0; split_any; ++round) {
         p.run = round < 12 ? (int)((max((int64_t)a.run_min, min(want, (int64_t)0x1fffffff)) + 63) / 64 * 64) : 0x3fffffff;
         int n = 0, split = 0;
         for (int u = lane; u < a.units; u += 64) {
-            const Unit x = unit_of(a, u);
+            const Unit x = u < 64 ? first : unit_of(a, u);
             const int runs = max(1, (int)(((int64_t)x.kv + p.run - 1) / p.run)), k = tiles_of<TILE>(a, x) * a.d.kv_heads * runs;
             n += k;
             if (runs > 1) split += k;
@@ -426,7 +439,7 @@ template <int TILE> DEVI Plan make_plan(const Args& a, int* lds) {
     }
     // longest first: workgroups that come free late then get short work (makespan over 6 requests of 1711 .. 16771 keys: 1.07 of the mean, 1.4 in any order)
     if (a.units <= 64) {
-        const int mine = lane < a.units ? unit_of(a, lane).kv : -1;
+        const int mine = lane < a.units ? first.kv : -1;
         int rank = 0;
 #pragma unroll 4
         for (int v = 0; v < a.units; ++v) {
@@ -475,7 +488,7 @@ DEVI int find(const int* first, int units, int i) {          // the last unit wh
 struct Item { int u, run, tile, head; Unit x; };
 template <int TILE> DEVI Item item_of(const Args& a, const Plan& plan, int item) {
     Item it;
-    if (a.split || TILE != STEP_ROWS) {
+    if (plan.split || TILE != STEP_ROWS) {
         it.u = find(plan.item0, a.units, item);
         it.x = unit_of(a, plan.order[it.u]);
         int rest = item - plan.item0[it.u];
@@ -536,7 +549,7 @@ __global__ __launch_bounds__(2 * chunk_rows<T>, D * (int)sizeof(T) >= 512 ? 1 : 
     extern __shared__ unsigned char lds[];
     constexpr int CHUNK_ROWS = chunk_rows<T>, NW = CHUNK_ROWS / 32, NS = chunk_subtiles<T>, KT = 32 * NS, RB = D * (int)sizeof(T), IMG = KT * RB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Plan plan = make_plan<CHUNK_ROWS>(a, reinterpret_cast<int*>(lds + 4 * IMG));
+    const Plan plan = make_plan<CHUNK_ROWS>(a, any_long(a), reinterpret_cast<int*>(lds + 4 * IMG));
     for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
         const Item it = item_of<CHUNK_ROWS>(a, plan, item);
         const Unit& x = it.x;
@@ -624,7 +637,7 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned char* mine = lds + wave * 2 * IMG;
     int* shared_to = reinterpret_cast<int*>(lds + 8 * IMG);
-    const Plan plan = make_plan<STEP_ROWS>(a, shared_to + 4);
+    const Plan plan = make_plan<STEP_ROWS>(a, any_long(a), shared_to + 4);
     for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
         const Item it = item_of<STEP_ROWS>(a, plan, item);
         const Unit& x = it.x;
@@ -753,7 +766,8 @@ __global__ __launch_bounds__(256, D * (int)sizeof(T) >= 512 ? 1 : 2) void paged_
 template <typename T, int D, int TILE>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(Args a) {
     extern __shared__ unsigned char lds[];
-    const Plan plan = make_plan<TILE>(a, reinterpret_cast<int*>(lds));
+    if (!any_long(a)) return;
+    const Plan plan = make_plan<TILE>(a, true, reinterpret_cast<int*>(lds));
     constexpr int PER = D / 4, ROWS = 256 / PER;                                 // threads per row, rows at a time
     constexpr int SLICES = TILE / ROWS;
     for (int i = blockIdx.x; i < plan.joins * SLICES; i += gridDim.x) {

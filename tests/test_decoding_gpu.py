@@ -207,6 +207,15 @@ def test_long_cache_few_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("beams,kv,new", [(1, [150, 1, 512], 1), (4, [150, 40], 1), (1, [150, 511, 70], 40), (1, [150, 513, 70], 1), (1, [100, 900, 70], 40), (4, [150, 700], 1)])
+def test_requests_in_tables_with_room_for_long_ones(dtype, beams, kv, new):
+    """Nothing is split where no request is long, whatever the tables have room for; one long request among short ones is."""
+    c = attend_case(kv, [new if n >= new else n for n in kv], beams=beams, heads=4, kv_heads=2, dim=64, dtype=dtype)
+    c["tables"] = torch.cat([c["tables"], torch.full((len(kv) * beams, 200), -1, dtype=I32, device=DEV)], 1)
+    attend_check(c, beams=beams)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_between_the_requests_and_a_token_major_pool(dtype):
     attend_check(attend_case([40, 3, 70], [7, 3, 40], heads=4, kv_heads=2, dim=64, dtype=dtype, token_major=True, gaps=3))
     attend_check(attend_case([40, 3, 70], [1, 1, 1], heads=4, kv_heads=2, dim=128, dtype=dtype, token_major=True, gaps=2))
