@@ -17,7 +17,7 @@
 //   long caches   8 requests of 16384 .. 65536 keys, 32 heads on 8, head_dim 128, one token: 191 us, 5.3 TB/s of pages.  Memory.
 //   steps         32 groups of 5 beams, 120 .. 181 keys of which the prompt's pages are shared, 12 heads of 64: 11.9 us for 21.5 MB.  The chain lengths, table,
 //                 first tile, four tiles, meeting of the waves; with every beam reading the shared pages itself 25.3 us.
-//   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 333 us, 810 TFLOP/s.  Products (512 cycles per 32 keys of a wave) and vector instructions (500) of
+//   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 340 us, 794 TFLOP/s (333 on another card).  Products (512 cycles per 32 keys of a wave) and vector instructions (500) of
 //                 the two waves that a SIMD holds; without exponentials it takes 320 us, without staging 293, without barriers too 280.
 //   fp32 prompts  32 prompts of 70 .. 170 tokens, 12 heads of 64: 35.6 us.  The products of the longest prompts (3.5 us per 32 keys for two waves on a SIMD) behind 10 us
 //                 of lengths, plan, queries, first tile and output.
@@ -495,8 +495,8 @@ template <int TILE> DEVI Item item_of(const Args& a, const Plan& plan, int item)
         it.head = rest % a.d.kv_heads;
         rest /= a.d.kv_heads;
         const int tiles = tiles_of<TILE>(a, it.x);
-        it.tile = rest % tiles;
         it.run = rest / tiles;
+        it.tile = tiles - 1 - (rest - it.run * tiles);                        // the last tokens, which see most, first (4096 tokens of one prompt: 220 -> 194 us)
     } else {
         it.u = item / a.d.kv_heads;
         it.head = item - it.u * a.d.kv_heads;
@@ -787,7 +787,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(Args a) {
             f32x4 v[AT_ONCE];
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
-                const int part = plan.part0[u] + (min(r0 + k, runs - 1) * tiles + tile) * a.d.kv_heads + h;
+                const int part = plan.part0[u] + (min(r0 + k, runs - 1) * tiles + tiles - 1 - tile) * a.d.kv_heads + h;
                 const float* ml = part_ml<D, TILE>(a, part) + 2 * at_row;
                 mr[k] = ml[0];
                 lr[k] = ml[1];
