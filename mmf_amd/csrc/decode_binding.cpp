@@ -265,19 +265,34 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
     return {o[0], o[1], o[2], o[3], o[4]};
 }
 
+// The planes of a cache are one run: a leading dimension steps over all planes of the dimension behind it, and of the next one that has several (what stands between,
+// of size 1, may have any stride).
+int64_t inner_plane_dim(const Tensor& c, int64_t a) {             // the next leading dimension behind a of a size other than 1; -1: none
+    for (++a; a <= c.dim() - 5; ++a)
+        if (c.size(a) != 1) return a;
+    return -1;
+}
 void check_planes(const Tensor& c) {
     check_float(c, "cache");
     NEED(c.dim() >= 4 && c.numel() > 0 && c.stride(-1) == 1, "cache must be [..., pages, kv_heads, page_size, head_dim] with contiguous head_dim, got ", c.sizes());
-    for (int64_t a = 0; a < c.dim() - 5; ++a)
-        NEED(c.size(a) == 1 || c.stride(a) == c.stride(a + 1) * c.size(a + 1), "the leading dimensions of cache must be one run of planes");
+    for (int64_t a = 0; a < c.dim() - 5; ++a) {
+        const int64_t in = inner_plane_dim(c, a);
+        NEED(c.size(a) == 1 || (c.stride(a) == c.stride(a + 1) * c.size(a + 1) && (in < 0 || c.stride(a) == c.stride(in) * c.size(in))),
+             "the leading dimensions of cache must be one run of planes");
+    }
     check_page(c.size(-2));
+}
+int64_t plane_step(const Tensor& c) {                             // from a plane to the next; 0: there is one
+    for (int64_t a = c.dim() - 5; a >= 0; --a)
+        if (c.size(a) != 1) return c.stride(a);
+    return 0;
 }
 void copy(const int32_t* copies, int64_t n, const Tensor& c, void* stream) {
     mmf_paged_copy_desc d = {};
     int64_t planes = 1;
     for (int64_t a = 0; a < c.dim() - 4; ++a) planes *= c.size(a);
     d.copies = copies; d.cache = P(c);
-    d.plane_stride = c.dim() > 4 ? step_of(c, c.dim() - 5) : 0;
+    d.plane_stride = plane_step(c);
     d.page_stride = step_of(c, c.dim() - 4); d.head_stride = step_of(c, c.dim() - 3); d.pos_stride = step_of(c, c.dim() - 2);
     NEED(n <= 0x7fffffff && planes <= 65535 && c.size(-4) <= 0x7fffffff, "too many rows or planes");
     d.rows = (int)n; d.planes = (int)planes; d.pages = (int)c.size(-4); d.page_size = (int)c.size(-2); d.kv_heads = (int)c.size(-3); d.head_dim = (int)c.size(-1);

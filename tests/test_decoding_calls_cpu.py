@@ -1,0 +1,41 @@
+"""What the decoding operators (mmf_amd/decoding.py) say about calls before any kernel runs: layouts, tangents, what a call writes."""
+import pytest
+import torch
+
+from mmf_amd import decoding as d
+
+I32, I64 = torch.int32, torch.int64
+
+
+def z(*s, dt=I32):
+    return torch.zeros(*s, dtype=dt)
+
+
+# ---------------------------------------------------------------------------------------------
+# planes
+# ---------------------------------------------------------------------------------------------
+PAGE = (4, 2, 16, 64)
+P = 4 * 2 * 16 * 64
+INNER = (2 * 16 * 64, 16 * 64, 64, 1)
+
+
+def planes(sizes, strides):
+    room = sum((n - 1) * s for n, s in zip(sizes, strides)) + P
+    return torch.zeros(room).as_strided((*sizes, *PAGE), (*strides, *INNER))
+
+
+@pytest.mark.parametrize("sizes,strides", [
+    ((3, 1, 2), (3 * P, 3 * P, P)),            # the middle one hides that the outer steps over more planes than the inner has
+    ((3, 1, 1, 2), (3 * P, 3 * P, 2 * P, P)), ((3, 2), (3 * P, P)), ((2, 3, 1, 2), (6 * P, 3 * P, 3 * P, P))])
+@pytest.mark.parametrize("call", ["copy", "reorder"])
+def test_planes_that_are_no_run_are_refused(sizes, strides, call):
+    cache = planes(sizes, strides)
+    with pytest.raises(RuntimeError, match="run of planes"):
+        d.copy_pages(z(4, 3), cache) if call == "copy" else d.reorder_pages(z(2, 3, dt=I64), z(2), z(6, 2), cache)
+
+
+@pytest.mark.parametrize("sizes,strides", [
+    ((3, 1), (P, P)), ((1, 3), (17, P)), ((3, 1, 2), (2 * P, 2 * P, P)), ((1, 1), (5, 7)), ((3,), (2 * P,)), ((), ()), ((1, 2, 1, 3), (9, 3 * P, 3 * P, P))])
+def test_planes_that_are_a_run_reach_the_device_check(sizes, strides):
+    with pytest.raises(RuntimeError, match="HBM"):
+        d.copy_pages(z(4, 3), planes(sizes, strides))
