@@ -816,6 +816,9 @@ typedef struct mmf_beam_select_desc {
 } mmf_beam_select_desc;
 int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab, int is_f32);
 int mmf_beam_select(const mmf_beam_select_desc* d, void* stream);
+/* The same with the history's column on the device: *step in the place of d->step, read by every replay of a captured call.  Outside 0 .. length - 1 it is reported, and
+ * the rows of the parents come back without the new tokens. */
+int mmf_beam_select_at(const mmf_beam_select_desc* d, const int32_t* step, void* stream);
 /* Tables after a selection: row w of a group becomes row parents[w]; the first child of a row keeps its unfinished block's page, every other child gets the page
  * of a row without children and a line in copies [groups * beams, 3] (source, destination, tokens; else -1) for mmf_paged_copy.  tables_out may be tables. */
 typedef struct mmf_paged_reorder_desc {

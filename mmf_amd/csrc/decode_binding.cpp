@@ -218,7 +218,8 @@ Tensor attend_pages(const Tensor& q, const Tensor& key_cache, const Tensor& valu
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& logits, const Tensor& scores, const Tensor& finished, int64_t eos,
-                                                                const optional<Tensor>& history_, int64_t step, at::TensorList out) {
+                                                                const optional<Tensor>& history_, int64_t step, const optional<Tensor>& step_at_,
+                                                                at::TensorList out) {
     check_dense(scores, "scores", at::kFloat, {-1, -1});
     const int64_t G = scores.size(0), W = scores.size(1);
     check_beams(W);
@@ -231,9 +232,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
     check_dense(finished, "finished", at::kBool, {G, W});
     NEED(eos >= 0 && eos < V, "eos ", eos, " is not in the vocabulary of ", V);
     const Tensor history = history_.has_value() ? *history_ : Tensor();
+    const Tensor step_at = step_at_.has_value() ? *step_at_ : Tensor();
+    if (step_at.defined()) check_dense(step_at, "step", at::kInt, {1});
     if (history.defined()) {
         check_dense(history, "history", at::kLong, {G, W, -1});
-        NEED(step >= 0 && step < history.size(2), "step ", step, " is not a column of the history of length ", history.size(2));
+        NEED(step_at.defined() || (step >= 0 && step < history.size(2)), "step ", step, " is not a column of the history of length ", history.size(2));
     }
     Tensor o[5];
     if (!out.empty()) {
@@ -243,7 +246,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
         for (int i = 0; i < 4; ++i) check_dense(o[i] = out[i], names[i], types[i], {G, W});
         if (history.defined()) check_dense(o[4] = out[4], "out.history", at::kLong, {G, W, history.size(2)});
     }
-    On on({&logits, &scores, &finished, &history, &o[0], &o[1], &o[2], &o[3], &o[4]});
+    On on({&logits, &scores, &finished, &history, &step_at, &o[0], &o[1], &o[2], &o[3], &o[4]});
     if (out.empty()) {
         Carver c(Carver::room(4 * G * W) + 2 * Carver::room(8 * G * W) + Carver::room(G * W), logits);
         o[0] = c.take({G, W}, at::kFloat);
@@ -260,7 +263,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
     d.ws = P(ws);
     d.vocab = V; d.eos = eos; d.length = history.defined() ? history.size(2) : 0; d.step = step;
     d.groups = (int)G; d.beams = (int)W; d.is_f32 = logits.scalar_type() == at::kFloat;
-    done(mmf_beam_select(&d, on.stream), "mmf_beam_select");
+    done(step_at.defined() ? mmf_beam_select_at(&d, PT<int32_t>(step_at), on.stream) : mmf_beam_select(&d, on.stream), "mmf_beam_select");
     if (!o[4].defined()) o[4] = at::empty({0}, o[1].options());
     return {o[0], o[1], o[2], o[3], o[4]};
 }
@@ -337,7 +340,8 @@ TORCH_LIBRARY(mmf_amd_decode, m) {
     m.def("write_pages(Tensor k, Tensor v, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots) -> ()");
     m.def("attend_pages(Tensor q, Tensor key_cache, Tensor value_cache, Tensor tables, Tensor kv_lens, Tensor q_start, Tensor q_lens, int max_q, int beams, bool causal, "
           "float? scale, Tensor? out) -> Tensor");
-    m.def("select_beams(Tensor logits, Tensor scores, Tensor finished, int eos, Tensor? history, int step, Tensor(a!)[] out) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("select_beams(Tensor logits, Tensor scores, Tensor finished, int eos, Tensor? history, int step, Tensor? step_at, "
+          "Tensor(a!)[] out) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("reorder_pages(Tensor parents, Tensor kv_lens, Tensor tables, Tensor(a!) cache, Tensor? out) -> Tensor");
     m.def("copy_pages(Tensor copies, Tensor(a!) cache) -> ()");
 }

@@ -446,7 +446,8 @@ __global__ __launch_bounds__(256, WIDE ? 8 : 4) void beam_rows_kernel(mmf_beam_s
     }
 }
 
-__global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d, int segments) {
+// step_at: the column of the new tokens where the host does not know it (a captured call that is replayed), else null
+__global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d, int segments, const int32_t* step_at) {
     __shared__ double cand_v[LIST], score[MMF_BEAMS_MAX], lse[MMF_BEAMS_MAX], best_v[MMF_BEAMS_MAX], red_v[4];
     __shared__ int64_t cand_i[LIST], best_i[MMF_BEAMS_MAX], red_i[4];
     __shared__ int done[MMF_BEAMS_MAX], parent[MMF_BEAMS_MAX], count;
@@ -463,6 +464,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
         best_i[tid] = -1;
     }
     if (tid == 0) count = 0;
+    const int64_t step = step_at ? *step_at : d.step;             // (read with the first loads; needed last)
     const int per = segments * W, cols = (int)min((int64_t)(LIST / W), d.length);
     const float one = 1.f / per, per_col = 1.f / cols;            // k / per for k < 2^20 (a vocabulary of 2^22): half a unit is more than the rounding
     auto beam_of = [&](int k) { return (int)(((float)k + 0.5f) * one); };
@@ -608,6 +610,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
     }
     __syncthreads();
     if (!d.history) return;
+    if (tid == 0 && (step < 0 || step >= d.length)) flag_page_error();       // (no column is the step's: the parents' rows come back as they are)
     // through LDS, many columns at a time: in place as well
     for (int64_t t0 = 0; t0 < d.length; t0 += cols) {
 #pragma unroll
@@ -624,7 +627,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(mmf_beam_select_desc d,
         for (int e = 0; e < KEEP; ++e) {
             const int k = tid + 256 * e, w = (int)(((float)k + 0.5f) * per_col);
             const int64_t t = t0 + k - w * cols;
-            if (k < W * cols && t < d.length) d.history_out[at + w * d.length + t] = t == d.step ? best_i[w] : cand_i[parent[w] * cols + k - w * cols];
+            if (k < W * cols && t < d.length) d.history_out[at + w * d.length + t] = t == step ? best_i[w] : cand_i[parent[w] * cols + k - w * cols];
         }
         __syncthreads();
     }
@@ -787,12 +790,12 @@ int64_t mmf_beam_select_ws_bytes(int groups, int beams, int64_t vocab, int is_f3
     return ((rows * n * beams + 1) & ~1ll) * (int64_t)sizeof(Picked) + rows * n * (int64_t)sizeof(Segment);
 }
 
-int mmf_beam_select(const mmf_beam_select_desc* d, void* stream) {
+static int beam_select(const mmf_beam_select_desc* d, const int32_t* step_at, void* stream) {
     MMF_CHECK_ARG(d && d->logits && d->scores && d->finished && d->scores_out && d->parents && d->tokens && d->finished_out && d->ws, "beam_select: null operand");
     MMF_CHECK_ARG(d->groups > 0 && d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->vocab > 0 && d->ld >= d->vocab, "beam_select: bad shape");
     MMF_CHECK_ARG(d->vocab <= 1 << 22 && (int64_t)d->groups * d->beams <= 65535, "beam_select: 2^22 tokens and 65535 rows at most");
     MMF_CHECK_ARG(d->eos >= 0 && d->eos < d->vocab, "beam_select: the end token is not in the vocabulary");
-    MMF_CHECK_ARG(!d->history || (d->history_out && d->length > 0 && d->step >= 0 && d->step < d->length), "beam_select: step is not a column of the history");
+    MMF_CHECK_ARG(!d->history || (d->history_out && d->length > 0 && (step_at || (d->step >= 0 && d->step < d->length))), "beam_select: step is not a column of the history");
     int length;
     const int segments = beam_segments(d->groups * d->beams, d->vocab, d->is_f32 != 0, &length);
     const dim3 grid(segments, d->groups * d->beams);
@@ -801,9 +804,16 @@ int mmf_beam_select(const mmf_beam_select_desc* d, void* stream) {
     else if (wide) hipLaunchKernelGGL((beam_rows_kernel<bf16, true>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
     else hipLaunchKernelGGL((beam_rows_kernel<bf16, false>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
     MMF_CHECK_LAUNCH();
-    hipLaunchKernelGGL(beam_merge_kernel, dim3(d->groups), dim3(256), 0, (hipStream_t)stream, *d, segments);
+    hipLaunchKernelGGL(beam_merge_kernel, dim3(d->groups), dim3(256), 0, (hipStream_t)stream, *d, segments, step_at);
     MMF_CHECK_LAUNCH();
     return 0;
+}
+
+int mmf_beam_select(const mmf_beam_select_desc* d, void* stream) { return beam_select(d, nullptr, stream); }
+
+int mmf_beam_select_at(const mmf_beam_select_desc* d, const int32_t* step, void* stream) {
+    MMF_CHECK_ARG(step, "beam_select: null operand");
+    return beam_select(d, step, stream);
 }
 
 int mmf_paged_reorder(const mmf_paged_reorder_desc* d, void* stream) {

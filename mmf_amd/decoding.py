@@ -12,8 +12,9 @@ The reference decodes M4C greedily by re-running the whole transformer (mmf/mode
 
 A cache pool is [pages, kv_heads, page_size, head_dim] (any strides with contiguous head_dim), page_size a power of two up to 1024, bf16 or fp32.  Requests come
 in groups of `beams` rows of the same length; a block table [groups * beams, blocks] int32 names the page of every block of a row.  Lengths stay on the device: no
-call here waits for the GPU, and every call can be captured into a hipGraph.  An index outside its table (a page, a slot, a parent) is left out and reported by
-`mmf_amd._native.take_index_error()`.  Forward only: tensors that require gradients are refused while gradients are on."""
+call here waits for the GPU, and every call can be captured into a hipGraph (its numbers with it: a selection that is replayed takes its `step` from the device).  An
+index outside its table (a page, a slot, a parent, a step) is left out and reported by `mmf_amd._native.take_index_error()`.  Forward only: tensors that require
+gradients are refused while gradients are on."""
 import os
 from collections import namedtuple
 
@@ -88,11 +89,13 @@ def select_beams(logits, scores, finished, *, eos, history=None, step=0, out=Non
     logits [groups * beams, vocab] bf16 or fp32 (contiguous rows; up to 2**22 tokens); scores fp32 [groups, beams]: the sums of log-probabilities so far, -inf for a beam that is not
     live (all but one before the first token); finished bool [groups, beams].  A candidate is scores + log_softmax(logits); a finished beam has one, the token `eos` at its
     score.  Descending, among equals the lowest beam * vocab + token first.  NaN counts as -inf; a row that holds +inf is all -inf.  history int64
-    [groups, beams, length]: the rows of the parents come back with the new tokens in column `step`.  `out`: a BeamStep whose tensors take the results; each may be the input
+    [groups, beams, length]: the rows of the parents come back with the new tokens in column `step`, a number or an int32 [1] tensor on the device; a number is
+    part of a captured call and stays what it was at capture, so a step that is replayed takes a tensor and advances it (`step += 1`).  `out`: a BeamStep whose tensors take the results; each may be the input
     of its kind."""
     if out is not None:
         out = [t for t in out if t is not None]
-    r = _lib().select_beams(logits, scores, finished, eos, history, step, out or [])
+    at = step if torch.is_tensor(step) else None
+    r = _lib().select_beams(logits, scores, finished, eos, history, 0 if at is not None else step, at, out or [])
     return BeamStep(*r) if history is not None else BeamStep(*r[:4], None)
 
 
@@ -114,7 +117,7 @@ def copy_pages(copies, cache):
 
 class PagedCache:
     """Pool, block tables, free list and lengths of a decoder with `layers` layers for `groups` requests of `beams` rows; every update is in place, so that a
-    step can be captured once and replayed.
+    step can be captured once and replayed (with `select_beams(..., step=at)`, `at` an int32 [1] tensor that the step advances).
 
         cache = PagedCache(layers, groups, beams, max_len, kv_heads=12, head_dim=64)
         plan = cache.plan(prompt_lens, rows, shared=True)         # the prompts: once per group

@@ -39,3 +39,19 @@ def test_planes_that_are_no_run_are_refused(sizes, strides, call):
 def test_planes_that_are_a_run_reach_the_device_check(sizes, strides):
     with pytest.raises(RuntimeError, match="HBM"):
         d.copy_pages(z(4, 3), planes(sizes, strides))
+
+
+# ---------------------------------------------------------------------------------------------
+# a step on the device
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("step,says", [(z(1), "HBM"), (z(1, dt=I64), "step must be"), (z(2), "step must be"), (torch.tensor(3, dtype=I32), "step must be"), (z(1).float(), "step must be"),
+                                       (5, "not a column"), (-1, "not a column")])
+def test_steps_that_are_no_column_and_no_int32_tensor_are_refused(step, says):
+    with pytest.raises(RuntimeError, match=says):
+        d.select_beams(torch.zeros(6, 10), torch.zeros(2, 3), z(2, 3, dt=torch.bool), eos=2, history=z(2, 3, 5, dt=I64), step=step)
+
+
+def test_the_c_entry_refuses_a_null_step():
+    from mmf_amd import _native as nat
+    L = nat.lib()
+    assert L.mmf_beam_select_at(None, None, None) != 0 and b"null operand" in L.mmf_amd_last_error()

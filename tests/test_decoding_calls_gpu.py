@@ -60,3 +60,77 @@ def test_planes_of_a_slice_of_the_layers():
     want[:, 0, 3, :, :7] = cache[:, 0, 0, :, :7]
     D().copy_pages(i32([[0, 3, 7]]), cache[:, 0])
     assert torch.equal(cache, want)
+
+
+# ---------------------------------------------------------------------------------------------
+# a step on the device
+# ---------------------------------------------------------------------------------------------
+def beam_state(G, W, V, length, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    scores = -torch.rand(G, W, generator=g).cumsum(1)
+    return (torch.randn(G * W, V, generator=g) * 2).to(DEV), scores.to(DEV), (torch.rand(G, W, generator=g) < 0.2).to(DEV), torch.randint(0, V, (G, W, length), generator=g).to(DEV)
+
+
+@pytest.mark.parametrize("length,beams", [(1, 3), (7, 1), (300, 5), (40, 32)])
+def test_a_step_on_the_device_is_the_same_number(length, beams):
+    x, s, f, h = beam_state(3, beams, 700, length)
+    for step in {0, length // 2, length - 1}:
+        want = D().select_beams(x, s, f, eos=2, history=h, step=step)
+        got = D().select_beams(x, s, f, eos=2, history=h, step=i32([step]))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(got.history[:, :, step], got.tokens)
+
+
+@pytest.mark.parametrize("step", [-1, 9, -2 ** 31, 2 ** 31 - 1])
+def test_a_step_outside_the_history_is_left_out_and_reported(step):
+    from mmf_amd import _native as nat
+    x, s, f, h = beam_state(2, 4, 500, 9)
+    want = D().select_beams(x, s, f, eos=2, history=h, step=0)
+    got = D().select_beams(x, s, f, eos=2, history=h, step=i32([step]))
+    assert nat.take_index_error()
+    assert all(torch.equal(a, b) for a, b in zip(got[:4], want[:4]))
+    assert torch.equal(got.history, h.gather(1, got.parents[:, :, None].expand_as(h)))
+    D().select_beams(x, s, f, eos=2, step=i32([step]))          # without a history there is no column to miss
+
+
+@pytest.mark.parametrize("beams,dtype", [(1, torch.bfloat16), (3, torch.bfloat16), (5, torch.float32)])
+def test_a_captured_search_keeps_its_tokens(beams, dtype):
+    """A step captured once and replayed, the history's column advanced within it: every column is the eager search's, after each replay."""
+    from tests.test_decoding_gpu import Decoder
+    d = D()
+    G, steps = 2, 9
+    model = Decoder(dtype=dtype, seed=4)
+    runs = []
+    for graphed in (False, True):
+        cache = d.PagedCache(model.layers, G, beams, 64, kv_heads=2, head_dim=64, page_size=8, dtype=dtype)
+        plan = cache.plan(i32([11, 6]), 17, shared=True)
+        g = torch.Generator().manual_seed(1)
+        logits = model.step(cache, plan, torch.randint(3, model.vocab, (17,), generator=g).to(DEV), 11)[torch.tensor([10, 16], device=DEV)].repeat_interleave(beams, 0)
+        scores = torch.full((G, beams), float("-inf"), device=DEV); scores[:, 0] = 0
+        b = d.select_beams(logits, scores, torch.zeros(G, beams, dtype=torch.bool, device=DEV), eos=2, history=torch.full((G, beams, steps), -1, device=DEV), step=0)
+        state, at, one = d.BeamStep(*(x.clone() for x in b)), i32([1]), torch.ones(G, dtype=I32, device=DEV)
+
+        def step(column):
+            cache.reorder(state.parents)
+            plan = cache.plan(one, G * beams)
+            logits = model.step(cache, plan, state.tokens.view(-1), 1)
+            d.select_beams(logits, state.scores, state.finished, eos=2, history=state.history, step=column, out=state)
+
+        step(at if graphed else 1)                             # warm: library handles, workspaces
+        at += 1
+        if graphed:
+            graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                step(at)
+                at += 1
+        seen = []
+        for i in range(2, steps):
+            graph.replay() if graphed else step(i)
+            junk = torch.randn(64, 64, device=DEV) @ torch.randn(64, 64, device=DEV)
+            torch.cuda.synchronize()
+            seen.append([x.clone() for x in state])
+            assert bool((state.history[:, :, :i + 1] >= 0).all()) and bool((state.history[:, :, i + 1:] == -1).all())
+        runs.append(seen)
+    for a, b in zip(*runs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
