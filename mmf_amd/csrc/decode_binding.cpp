@@ -2,6 +2,7 @@
 // Every argument check of these operators is here, so that a call costs the host a few microseconds: a decoding step is a handful of kernels of about as many.
 // The library loads without a GPU as well; the operators then refuse (no CPU path).
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -22,6 +23,7 @@ using std::optional;
 void check(const Tensor& t, const char* name, at::ScalarType dt) {
     NEED(t.scalar_type() == dt, name, " must be ", dt, ", got ", t.scalar_type());
     NEED(!(t.requires_grad() && at::GradMode::is_enabled()), name, " requires a gradient: decoding is forward only (torch.no_grad)");
+    NEED(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), name, " carries a tangent: decoding has no derivative in forward mode");
 }
 void check_float(const Tensor& t, const char* name) {
     NEED(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, name, " must be bfloat16 or float32, got ", t.scalar_type());

@@ -14,7 +14,7 @@ A cache pool is [pages, kv_heads, page_size, head_dim] (any strides with contigu
 in groups of `beams` rows of the same length; a block table [groups * beams, blocks] int32 names the page of every block of a row.  Lengths stay on the device: no
 call here waits for the GPU, and every call can be captured into a hipGraph (its numbers with it: a selection that is replayed takes its `step` from the device).  An
 index outside its table (a page, a slot, a parent, a step) is left out and reported by `mmf_amd._native.take_index_error()`.  Forward only: tensors that require
-gradients are refused while gradients are on."""
+gradients are refused while gradients are on, and so are those that carry a tangent of forward-mode differentiation."""
 import os
 from collections import namedtuple
 

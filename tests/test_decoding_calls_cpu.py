@@ -55,3 +55,46 @@ def test_the_c_entry_refuses_a_null_step():
     from mmf_amd import _native as nat
     L = nat.lib()
     assert L.mmf_beam_select_at(None, None, None) != 0 and b"null operand" in L.mmf_amd_last_error()
+
+
+# ---------------------------------------------------------------------------------------------
+# forward-mode tangents: no operator here has a derivative
+# ---------------------------------------------------------------------------------------------
+bf = torch.bfloat16
+
+
+def calls():
+    kc, vc = torch.zeros(4, 2, 16, 64, dtype=bf), torch.zeros(4, 2, 16, 64, dtype=bf)
+    q, k = torch.zeros(9, 4, 64, dtype=bf), torch.zeros(5, 2, 64, dtype=bf)
+    attend = dict(q=q, key_cache=kc, value_cache=vc, tables=z(6, 3), kv_lens=z(3), q_start=z(6), q_lens=z(3), max_q=2, beams=2, out=torch.zeros(9, 4, 64, dtype=bf))
+    select = dict(logits=torch.zeros(6, 10), scores=torch.zeros(2, 3), finished=z(2, 3, dt=torch.bool), eos=2)
+    return {"write": (d.write_pages, dict(k=k, v=k.clone(), key_cache=kc, value_cache=vc, slots=z(5, dt=I64)), ("k", "v", "key_cache", "value_cache")),
+            "attend": (d.attend_pages, attend, ("q", "key_cache", "value_cache", "out")), "select": (d.select_beams, select, ("logits", "scores")),
+            "reorder": (d.reorder_pages, dict(parents=z(2, 3, dt=I64), kv_lens=z(2), tables=z(6, 2), cache=torch.zeros(3, 2, 4, 2, 16, 64)), ("cache",)),
+            "copy": (d.copy_pages, dict(copies=z(4, 3), cache=torch.zeros(3, 2, 4, 2, 16, 64)), ("cache",))}
+
+
+@pytest.mark.parametrize("call,name", [(c, n) for c, (_, _, names) in calls().items() for n in names])
+def test_tensors_with_tangents_are_refused_like_those_that_require_gradients(call, name):
+    import torch.autograd.forward_ad as fw
+    f, args, _ = calls()[call]
+    with fw.dual_level():
+        dual = fw.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(RuntimeError, match="%s carries a tangent" % name):
+            f(**dict(args, **{name: dual}))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="%s carries a tangent" % name):       # (no_grad stops the backward mode only)
+            f(**dict(args, **{name: dual}))
+        with fw._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="HBM"):
+            f(**dict(args, **{name: dual}))
+        with pytest.raises(RuntimeError, match="HBM"):
+            f(**dict(args, **{name: fw.unpack_dual(dual).primal}))
+    with pytest.raises(RuntimeError, match="%s requires a gradient" % name):
+        f(**dict(args, **{name: args[name].clone().requires_grad_(True)}))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="HBM"):
+        f(**dict(args, **{name: args[name].clone().requires_grad_(True)}))
+
+
+def test_tangents_of_function_transforms_are_refused():
+    f, args, _ = calls()["select"]
+    with pytest.raises(RuntimeError, match="logits carries a tangent"):
+        torch.func.jvp(lambda x: f(**dict(args, logits=x)).scores, (args["logits"],), (torch.ones_like(args["logits"]),))
