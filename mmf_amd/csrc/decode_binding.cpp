@@ -93,8 +93,9 @@ template <typename T> T* PT(const Tensor& t) { return static_cast<T*>(P(t)); }
 
 using Plan = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-Plan plan_pages(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& tables, const Tensor& owned, const Tensor& free_pages, const Tensor& free_top, int64_t page_size,
-                int64_t rows, int64_t beams, bool shared, at::TensorList out) {
+// out: where the results go, all or (null) none of them
+Plan plan_into(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& tables, const Tensor& owned, const Tensor& free_pages, const Tensor& free_top, int64_t page_size,
+               int64_t rows, int64_t beams, bool shared, const Plan* out) {
     check_page(page_size);
     check_beams(beams);
     check_dense(q_lens, "q_lens", at::kInt, {-1});
@@ -108,25 +109,23 @@ Plan plan_pages(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& table
     NEED(tables.size(1) > 0 && free_pages.numel() > 0, "tables and free_pages must not be empty");
     NEED(tables.size(1) * page_size <= (1 << 30) && R <= 0x0fffffff && free_pages.numel() <= 0x7fffffff, "a table row names more than 2**30 tokens");
     Plan p;
-    if (!out.empty()) {
-        NEED(out.size() == 8, "out is a PagePlan");
-        check_dense(out[0], "out.q_start", at::kInt, {n});
-        check_dense(out[1], "out.q_lens", at::kInt, {G});
-        check_dense(out[2], "out.kv_lens", at::kInt, {G});
-        check_dense(out[3], "out.slots", at::kLong, {rows});
-        check_dense(out[4], "out.positions", at::kInt, {rows});
-        check_dense(out[5], "out.copies", at::kInt, {R, 3});
-        check_dense(out[6], "out.free_top", at::kInt, {1});
-        check_dense(out[7], "out.refused", at::kInt, {1});
-        p = {out[0], out[1], out[2], out[3], out[4], out[5], out[6], out[7]};
+    if (out) {
+        p = *out;
+        check_dense(std::get<0>(p), "out.q_start", at::kInt, {n});
+        check_dense(std::get<1>(p), "out.q_lens", at::kInt, {G});
+        check_dense(std::get<2>(p), "out.kv_lens", at::kInt, {G});
+        check_dense(std::get<3>(p), "out.slots", at::kLong, {rows});
+        check_dense(std::get<4>(p), "out.positions", at::kInt, {rows});
+        check_dense(std::get<5>(p), "out.copies", at::kInt, {R, 3});
+        check_dense(std::get<6>(p), "out.free_top", at::kInt, {1});
+        check_dense(std::get<7>(p), "out.refused", at::kInt, {1});
     }
-    const Tensor none;
-    auto o = [&](size_t i) -> const Tensor* { return out.empty() ? &none : &out[i]; };
-    On on({&q_lens, &kv_lens, &tables, &owned, &free_pages, &free_top, o(0), o(1), o(2), o(3), o(4), o(5), o(6), o(7)});
+    On on({&q_lens, &kv_lens, &tables, &owned, &free_pages, &free_top, &std::get<0>(p), &std::get<1>(p), &std::get<2>(p), &std::get<3>(p), &std::get<4>(p), &std::get<5>(p),
+           &std::get<6>(p), &std::get<7>(p)});
     const int64_t ws_bytes = mmf_paged_plan_ws_bytes((int)G, (int)beams);
     void* ws;                                                     // (small: next to the results it costs no allocation of its own)
     Tensor ws_owner;
-    if (out.empty()) {
+    if (!out) {
         Carver c(Carver::room(ws_bytes) + Carver::room(8 * rows) + Carver::room(4 * n) + 2 * Carver::room(4 * G) + Carver::room(4 * rows) + Carver::room(12 * R) + 32, q_lens);
         ws = c.base.data_ptr();
         c.at = Carver::room(ws_bytes);
@@ -147,6 +146,16 @@ Plan plan_pages(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& table
     d.free_capacity = (int)free_pages.numel();
     done(mmf_paged_plan(&d, on.stream), "mmf_paged_plan");
     return p;
+}
+Plan plan_pages(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& tables, const Tensor& owned, const Tensor& free_pages, const Tensor& free_top, int64_t page_size,
+                int64_t rows, int64_t beams, bool shared) {
+    return plan_into(q_lens, kv_lens, tables, owned, free_pages, free_top, page_size, rows, beams, shared, nullptr);
+}
+void plan_pages_out(const Tensor& q_lens, const Tensor& kv_lens, const Tensor& tables, const Tensor& owned, const Tensor& free_pages, const Tensor& free_top, int64_t page_size,
+                    int64_t rows, int64_t beams, bool shared, const Tensor& q_start, const Tensor& granted, const Tensor& kv_out, const Tensor& slots, const Tensor& positions,
+                    const Tensor& copies, const Tensor& top_out, const Tensor& refused) {
+    const Plan out(q_start, granted, kv_out, slots, positions, copies, top_out, refused);
+    plan_into(q_lens, kv_lens, tables, owned, free_pages, free_top, page_size, rows, beams, shared, &out);
 }
 
 void write_pages(const Tensor& k, const Tensor& v, const Tensor& key_cache, const Tensor& value_cache, const Tensor& slots) {
@@ -174,8 +183,8 @@ void write_pages(const Tensor& k, const Tensor& v, const Tensor& key_cache, cons
     if (T) done(mmf_paged_write(&d, on.stream), "mmf_paged_write");
 }
 
-Tensor attend_pages(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache, const Tensor& tables, const Tensor& kv_lens, const Tensor& q_start,
-                    const Tensor& q_lens, int64_t max_q, int64_t beams, bool causal, optional<double> scale, const optional<Tensor>& out_) {
+Tensor attend_into(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache, const Tensor& tables, const Tensor& kv_lens, const Tensor& q_start,
+                   const Tensor& q_lens, int64_t max_q, int64_t beams, bool causal, optional<double> scale, Tensor out) {
     check_pools(key_cache, value_cache);
     const int64_t D = key_cache.size(3), Hk = key_cache.size(1);
     NEED(D == 64 || D == 128, "head_dim must be 64 or 128, got ", D);
@@ -193,7 +202,6 @@ Tensor attend_pages(const Tensor& q, const Tensor& key_cache, const Tensor& valu
          "], contiguous head_dim, heads a multiple of ", Hk, "; got ", q.sizes());
     NEED(max_q >= 1, "max_q must be at least 1, got ", max_q);
     NEED(on16(q, 2) && on16(key_cache, 3) && on16(value_cache, 3), "q, key_cache and value_cache must start and stride on 16 bytes");
-    Tensor out = out_.has_value() ? *out_ : Tensor();
     if (out.defined()) {
         check(out, "out", q.scalar_type());
         NEED(out.sizes() == q.sizes() && out.stride(2) == 1 && on16(out, 2), "out must be shaped as q, with contiguous head_dim, and start and stride on 16 bytes");
@@ -218,10 +226,20 @@ Tensor attend_pages(const Tensor& q, const Tensor& key_cache, const Tensor& valu
     done(mmf_paged_attention(&d, on.stream), "mmf_paged_attention");
     return out;
 }
+Tensor attend_pages(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache, const Tensor& tables, const Tensor& kv_lens, const Tensor& q_start,
+                    const Tensor& q_lens, int64_t max_q, int64_t beams, bool causal, optional<double> scale) {
+    return attend_into(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, max_q, beams, causal, scale, Tensor());
+}
+void attend_pages_out(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache, const Tensor& tables, const Tensor& kv_lens, const Tensor& q_start,
+                      const Tensor& q_lens, int64_t max_q, int64_t beams, bool causal, optional<double> scale, const Tensor& out) {
+    attend_into(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, max_q, beams, causal, scale, out);
+}
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& logits, const Tensor& scores, const Tensor& finished, int64_t eos,
-                                                                const optional<Tensor>& history_, int64_t step, const optional<Tensor>& step_at_,
-                                                                at::TensorList out) {
+using Beams = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+// out: where the results go, all (the history where there is one) or (null) none of them
+Beams select_into(const Tensor& logits, const Tensor& scores, const Tensor& finished, int64_t eos, const optional<Tensor>& history_, int64_t step,
+                  const optional<Tensor>& step_at_, const Tensor* const* out) {
     check_dense(scores, "scores", at::kFloat, {-1, -1});
     const int64_t G = scores.size(0), W = scores.size(1);
     check_beams(W);
@@ -241,15 +259,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
         NEED(step_at.defined() || (step >= 0 && step < history.size(2)), "step ", step, " is not a column of the history of length ", history.size(2));
     }
     Tensor o[5];
-    if (!out.empty()) {
-        NEED(out.size() == (history.defined() ? 5u : 4u), "out is a BeamStep; its history goes with history");
+    if (out) {
+        NEED(out[4]->defined() == history.defined(), "out is a BeamStep; its history goes with history");
         const char* names[4] = {"out.scores", "out.parents", "out.tokens", "out.finished"};
         const at::ScalarType types[4] = {at::kFloat, at::kLong, at::kLong, at::kBool};
-        for (int i = 0; i < 4; ++i) check_dense(o[i] = out[i], names[i], types[i], {G, W});
-        if (history.defined()) check_dense(o[4] = out[4], "out.history", at::kLong, {G, W, history.size(2)});
+        for (int i = 0; i < 4; ++i) check_dense(o[i] = *out[i], names[i], types[i], {G, W});
+        if (history.defined()) check_dense(o[4] = *out[4], "out.history", at::kLong, {G, W, history.size(2)});
     }
     On on({&logits, &scores, &finished, &history, &step_at, &o[0], &o[1], &o[2], &o[3], &o[4]});
-    if (out.empty()) {
+    if (!out) {
         Carver c(Carver::room(4 * G * W) + 2 * Carver::room(8 * G * W) + Carver::room(G * W), logits);
         o[0] = c.take({G, W}, at::kFloat);
         o[1] = c.take({G, W}, at::kLong);
@@ -268,6 +286,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> select_beams(const Tensor& lo
     done(step_at.defined() ? mmf_beam_select_at(&d, PT<int32_t>(step_at), on.stream) : mmf_beam_select(&d, on.stream), "mmf_beam_select");
     if (!o[4].defined()) o[4] = at::empty({0}, o[1].options());
     return {o[0], o[1], o[2], o[3], o[4]};
+}
+Beams select_beams(const Tensor& logits, const Tensor& scores, const Tensor& finished, int64_t eos, const optional<Tensor>& history, int64_t step,
+                   const optional<Tensor>& step_at) {
+    return select_into(logits, scores, finished, eos, history, step, step_at, nullptr);
+}
+void select_beams_out(const Tensor& logits, const Tensor& scores, const Tensor& finished, int64_t eos, const optional<Tensor>& history, int64_t step,
+                      const optional<Tensor>& step_at, const Tensor& scores_out, const Tensor& parents, const Tensor& tokens, const Tensor& finished_out,
+                      const optional<Tensor>& history_out) {
+    const Tensor none;
+    const Tensor* out[5] = {&scores_out, &parents, &tokens, &finished_out, history_out.has_value() ? &*history_out : &none};
+    select_into(logits, scores, finished, eos, history, step, step_at, out);
 }
 
 // The planes of a cache are one run: a leading dimension steps over all planes of the dimension behind it, and of the next one that has several (what stands between,
@@ -305,7 +334,7 @@ void copy(const int32_t* copies, int64_t n, const Tensor& c, void* stream) {
     done(mmf_paged_copy(&d, stream), "mmf_paged_copy");
 }
 
-Tensor reorder_pages(const Tensor& parents, const Tensor& kv_lens, const Tensor& tables, const Tensor& cache, const optional<Tensor>& out_) {
+Tensor reorder_into(const Tensor& parents, const Tensor& kv_lens, const Tensor& tables, const Tensor& cache, Tensor out) {
     check_dense(parents, "parents", at::kLong, {-1, -1});
     const int64_t G = parents.size(0), W = parents.size(1);
     check_beams(W);
@@ -314,7 +343,6 @@ Tensor reorder_pages(const Tensor& parents, const Tensor& kv_lens, const Tensor&
     check_dense(tables, "tables", at::kInt, {G * W, -1});
     NEED(tables.size(1) > 0 && tables.size(1) <= 0x3fffffff, "tables must not be empty");
     check_planes(cache);
-    Tensor out = out_.has_value() ? *out_ : Tensor();
     if (out.defined()) check_dense(out, "out", at::kInt, {G * W, tables.size(1)});
     On on({&parents, &kv_lens, &tables, &cache, &out});
     if (!out.defined()) out = at::empty(tables.sizes(), tables.options());
@@ -326,6 +354,12 @@ Tensor reorder_pages(const Tensor& parents, const Tensor& kv_lens, const Tensor&
     copy(d.copies, G * W, cache, on.stream);
     return out;
 }
+Tensor reorder_pages(const Tensor& parents, const Tensor& kv_lens, const Tensor& tables, const Tensor& cache) {
+    return reorder_into(parents, kv_lens, tables, cache, Tensor());
+}
+void reorder_pages_out(const Tensor& parents, const Tensor& kv_lens, const Tensor& tables, const Tensor& cache, const Tensor& out) {
+    reorder_into(parents, kv_lens, tables, cache, out);
+}
 
 void copy_pages(const Tensor& copies, const Tensor& cache) {
     check_dense(copies, "copies", at::kInt, {-1, 3});
@@ -336,23 +370,35 @@ void copy_pages(const Tensor& copies, const Tensor& cache) {
 
 }  // namespace
 
+// A schema marks every tensor that its call writes: the state that plans and copies change, and in the forms with `out` the results, which may be the inputs of their kind.
+// The results that a call makes itself are tensors of their own (several in one allocation, apart from each other).
+#define PLAN_ARGS "Tensor q_lens, Tensor kv_lens, Tensor(a!) tables, Tensor(b!) owned, Tensor(c!) free_pages, Tensor free_top, int page_size, int rows, int beams, bool shared"
+#define ATTEND_ARGS "Tensor q, Tensor key_cache, Tensor value_cache, Tensor tables, Tensor kv_lens, Tensor q_start, Tensor q_lens, int max_q, int beams, bool causal, float? scale"
+#define SELECT_ARGS "Tensor logits, Tensor scores, Tensor finished, int eos, Tensor? history, int step, Tensor? step_at"
 TORCH_LIBRARY(mmf_amd_decode, m) {
-    m.def("plan_pages(Tensor q_lens, Tensor kv_lens, Tensor(a!) tables, Tensor(b!) owned, Tensor(c!) free_pages, Tensor free_top, int page_size, int rows, int beams, "
-          "bool shared, Tensor(d!)[] out) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("plan_pages(" PLAN_ARGS ") -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("plan_pages.out(" PLAN_ARGS ", *, Tensor(d!) out_q_start, Tensor(e!) out_q_lens, Tensor(f!) out_kv_lens, Tensor(g!) out_slots, Tensor(h!) out_positions, "
+          "Tensor(i!) out_copies, Tensor(j!) out_free_top, Tensor(k!) out_refused) -> ()");
     m.def("write_pages(Tensor k, Tensor v, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots) -> ()");
-    m.def("attend_pages(Tensor q, Tensor key_cache, Tensor value_cache, Tensor tables, Tensor kv_lens, Tensor q_start, Tensor q_lens, int max_q, int beams, bool causal, "
-          "float? scale, Tensor? out) -> Tensor");
-    m.def("select_beams(Tensor logits, Tensor scores, Tensor finished, int eos, Tensor? history, int step, Tensor? step_at, "
-          "Tensor(a!)[] out) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
-    m.def("reorder_pages(Tensor parents, Tensor kv_lens, Tensor tables, Tensor(a!) cache, Tensor? out) -> Tensor");
+    m.def("attend_pages(" ATTEND_ARGS ") -> Tensor");
+    m.def("attend_pages.out(" ATTEND_ARGS ", *, Tensor(a!) out) -> ()");
+    m.def("select_beams(" SELECT_ARGS ") -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("select_beams.out(" SELECT_ARGS ", *, Tensor(a!) out_scores, Tensor(b!) out_parents, Tensor(c!) out_tokens, Tensor(d!) out_finished, "
+          "Tensor(e!)? out_history) -> ()");
+    m.def("reorder_pages(Tensor parents, Tensor kv_lens, Tensor tables, Tensor(a!) cache) -> Tensor");
+    m.def("reorder_pages.out(Tensor parents, Tensor kv_lens, Tensor tables, Tensor(a!) cache, *, Tensor(b!) out) -> ()");
     m.def("copy_pages(Tensor copies, Tensor(a!) cache) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(mmf_amd_decode, CompositeImplicitAutograd, m) {
     m.impl("plan_pages", plan_pages);
+    m.impl("plan_pages.out", plan_pages_out);
     m.impl("write_pages", write_pages);
     m.impl("attend_pages", attend_pages);
+    m.impl("attend_pages.out", attend_pages_out);
     m.impl("select_beams", select_beams);
+    m.impl("select_beams.out", select_beams_out);
     m.impl("reorder_pages", reorder_pages);
+    m.impl("reorder_pages.out", reorder_pages_out);
     m.impl("copy_pages", copy_pages);
 }

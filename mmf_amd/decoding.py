@@ -45,8 +45,9 @@ def _lib():
             raise nat.NativeLibraryError("mmf_amd decoding library not found at %s. Build it with `python -m mmf_amd.csrc.build`. There is no fallback path." % _LIB_PATH)
         torch.ops.load_library(_LIB_PATH)
         ns = torch.ops.mmf_amd_decode
-        _ops = namedtuple("Ops", "plan_pages write_pages attend_pages select_beams reorder_pages copy_pages")(
-            *(getattr(ns, n).default for n in ("plan_pages", "write_pages", "attend_pages", "select_beams", "reorder_pages", "copy_pages")))
+        forms = dict({n: getattr(ns, n).default for n in ("plan_pages", "write_pages", "attend_pages", "select_beams", "reorder_pages", "copy_pages")},
+                     **{n + "_out": getattr(ns, n).out for n in ("plan_pages", "attend_pages", "select_beams", "reorder_pages")})
+        _ops = namedtuple("Ops", forms)(**forms)
     return _ops
 
 
@@ -61,8 +62,14 @@ def plan_pages(q_lens, kv_lens, tables, owned, free_pages, free_top, *, page_siz
     A group is served whole or waits (no page, no slot, q_lens 0): when its tokens do not fit its table row or `rows`, or when it and the groups before it need
     more pages than are free.  Not shared, a row that still shares the block it goes on writing gets a page of its own and a line in `copies`: call
     `copy_pages(plan.copies, cache)` before the write.  `out`: a PagePlan whose tensors take the results; its kv_lens and free_top may be the inputs."""
-    return PagePlan(*_lib().plan_pages(q_lens, kv_lens, tables, owned, free_pages, free_top, page_size, rows, beams, shared, [] if out is None else list(out[:8])),
-                    1 if shared else beams)
+    if out is None:
+        return PagePlan(*_lib().plan_pages(q_lens, kv_lens, tables, owned, free_pages, free_top, page_size, rows, beams, shared), 1 if shared else beams)
+    if len(out) < 8:
+        raise nat.NativeLibraryError("out must be a PagePlan, got %d tensors" % len(out))
+    start, lens, kv, slots, positions, copies, top, refused = out[:8]
+    _lib().plan_pages_out(q_lens, kv_lens, tables, owned, free_pages, free_top, page_size, rows, beams, shared, out_q_start=start, out_q_lens=lens, out_kv_lens=kv,
+                          out_slots=slots, out_positions=positions, out_copies=copies, out_free_top=top, out_refused=refused)
+    return PagePlan(start, lens, kv, slots, positions, copies, top, refused, 1 if shared else beams)
 
 
 def write_pages(k, v, key_cache, value_cache, slots):
@@ -80,7 +87,10 @@ def attend_pages(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, *,
     (contiguous rows); kv_lens, q_lens int32 [requests // beams], q_start int32 [requests].  max_q: no request has more new tokens (tokens beyond are left out and
     reported).  scale: default head_dim ** -0.5.  A token that sees no key gives zeros; rows of `out` that no request names are left as they are (undefined
     where `out` is made here).  `out` may be q.  A page outside the pool reads as zeros and is reported."""
-    return _lib().attend_pages(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, max_q, beams, causal, scale, out)
+    if out is None:
+        return _lib().attend_pages(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, max_q, beams, causal, scale)
+    _lib().attend_pages_out(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, max_q, beams, causal, scale, out=out)
+    return out
 
 
 def select_beams(logits, scores, finished, *, eos, history=None, step=0, out=None):
@@ -92,11 +102,17 @@ def select_beams(logits, scores, finished, *, eos, history=None, step=0, out=Non
     [groups, beams, length]: the rows of the parents come back with the new tokens in column `step`, a number or an int32 [1] tensor on the device; a number is
     part of a captured call and stays what it was at capture, so a step that is replayed takes a tensor and advances it (`step += 1`).  `out`: a BeamStep whose tensors take the results; each may be the input
     of its kind."""
-    if out is not None:
-        out = [t for t in out if t is not None]
     at = step if torch.is_tensor(step) else None
-    r = _lib().select_beams(logits, scores, finished, eos, history, 0 if at is not None else step, at, out or [])
-    return BeamStep(*r) if history is not None else BeamStep(*r[:4], None)
+    step = 0 if at is not None else step
+    if out is None:
+        r = _lib().select_beams(logits, scores, finished, eos, history, step, at)
+        return BeamStep(*r) if history is not None else BeamStep(*r[:4], None)
+    if not 4 <= len(out) <= 5:
+        raise nat.NativeLibraryError("out must be a BeamStep, got %d tensors" % len(out))
+    out = BeamStep(*out[:4], out[4] if len(out) == 5 else None)
+    _lib().select_beams_out(logits, scores, finished, eos, history, step, at, out_scores=out.scores, out_parents=out.parents, out_tokens=out.tokens,
+                            out_finished=out.finished, out_history=out.history)
+    return out
 
 
 def reorder_pages(parents, kv_lens, tables, cache, *, out=None):
@@ -106,7 +122,10 @@ def reorder_pages(parents, kv_lens, tables, cache, *, out=None):
     head_dim]: every pool the tables are for (keys and values of all layers), leading dimensions as one contiguous run of planes.  Full blocks are shared by the children
     of a beam.  The block that goes on being written stays with the first child; the other children take the pages of beams without children and get its
     tokens copied in.  Returns the new tables (`out` may be `tables`)."""
-    return _lib().reorder_pages(parents, kv_lens, tables, cache, out)
+    if out is None:
+        return _lib().reorder_pages(parents, kv_lens, tables, cache)
+    _lib().reorder_pages_out(parents, kv_lens, tables, cache, out=out)
+    return out
 
 
 def copy_pages(copies, cache):

@@ -98,3 +98,48 @@ def test_tangents_of_function_transforms_are_refused():
     f, args, _ = calls()["select"]
     with pytest.raises(RuntimeError, match="logits carries a tangent"):
         torch.func.jvp(lambda x: f(**dict(args, logits=x)).scores, (args["logits"],), (torch.ones_like(args["logits"]),))
+
+
+# ---------------------------------------------------------------------------------------------
+# schemas: what a call writes is marked, and what it returns is its own
+# ---------------------------------------------------------------------------------------------
+STATE = {"plan_pages": {"tables", "owned", "free_pages"}, "write_pages": {"key_cache", "value_cache"}, "attend_pages": set(), "select_beams": set(), "reorder_pages": {"cache"},
+         "copy_pages": {"cache"}}
+
+
+@pytest.mark.parametrize("name", STATE)
+def test_schemas_mark_what_a_call_writes(name):
+    d._lib()
+    packet = getattr(torch.ops.mmf_amd_decode, name)
+    forms = {"default": STATE[name]}
+    if "out" in packet.overloads():
+        forms["out"] = STATE[name] | {a.name for a in packet.out._schema.arguments if a.name.startswith("out")}
+    assert ("out" in forms) == (name in ("plan_pages", "attend_pages", "select_beams", "reorder_pages"))
+    for form, written in forms.items():
+        schema = getattr(packet, form)._schema
+        assert {a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write} == written
+        assert all(r.alias_info is None for r in schema.returns)
+        assert not any(a.name.startswith("out") for a in schema.arguments) or (form == "out" and len(schema.returns) == 0)
+
+
+@pytest.mark.parametrize("call,out,says", [
+    ("select", (torch.zeros(2, 3),), "BeamStep"), ("select", (torch.zeros(2, 3), z(2, 3, dt=I64), z(2, 3, dt=I64), z(2, 3, dt=torch.bool)), "HBM"),
+    ("select", (torch.zeros(2, 3), z(2, 3, dt=I64), z(2, 3, dt=I64), z(2, 3, dt=torch.bool), z(2, 3, 4, dt=I64)), "history goes with history"),
+    ("select", (torch.zeros(2, 4), z(2, 3, dt=I64), z(2, 3, dt=I64), z(2, 3, dt=torch.bool)), "out.scores"), ("attend", torch.zeros(9, 4, 32, dtype=bf), "out must be"),
+    ("attend", torch.zeros(9, 4, 64), "out must be"), ("reorder", z(6, 3), "out must be")])
+def test_results_of_another_shape_or_kind_are_refused(call, out, says):
+    f, args, _ = calls()[call]
+    with pytest.raises(RuntimeError, match=says):
+        f(**dict(args, out=out))
+
+
+def test_a_plan_takes_a_whole_plan_of_results():
+    args = dict(q_lens=z(2), kv_lens=z(2), tables=z(6, 4), owned=z(6, 4), free_pages=z(9), free_top=z(1), page_size=16, rows=8, beams=3)
+    with pytest.raises(RuntimeError, match="PagePlan"):
+        d.plan_pages(**args, out=(z(6), z(2)))
+    good = [z(6), z(2), z(2), z(8, dt=I64), z(8), z(6, 3), z(1), z(1)]
+    for i, name in enumerate(d.PagePlan._fields[:8]):
+        bad = list(good)
+        bad[i] = z(11, dt=bad[i].dtype)
+        with pytest.raises(RuntimeError, match="out.%s must be" % name):
+            d.plan_pages(**args, out=bad)

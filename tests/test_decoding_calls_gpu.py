@@ -134,3 +134,51 @@ def test_a_captured_search_keeps_its_tokens(beams, dtype):
         runs.append(seen)
     for a, b in zip(*runs):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ---------------------------------------------------------------------------------------------
+# schemas
+# ---------------------------------------------------------------------------------------------
+def form_args():
+    g = torch.Generator().manual_seed(2)
+    kc, vc = (torch.randn(9, 2, 16, 64, generator=g).to(DEV) for _ in range(2))
+    q, k, v = (torch.randn(4, n, 64, generator=g).to(DEV) for n in (4, 2, 2))
+    x, s, f, h = beam_state(2, 2, 50, 6)
+    tables, owned = i32([[0, 1, -1], [0, 2, -1], [3, -1, -1], [3, -1, -1]]), i32([[0, 1, -1], [-1, 2, -1], [3, -1, -1], [-1, -1, -1]])
+    one = torch.ones(2, dtype=I32, device=DEV)
+    plan = dict(q_lens=one, kv_lens=i32([20, 16]), tables=tables.clone(), owned=owned, free_pages=i32([4, 5, 6, 7, 8]), free_top=i32([5]), page_size=16, rows=4, beams=2, shared=False)
+    attend = dict(q=q, key_cache=kc, value_cache=vc, tables=tables[:, :2].clamp(min=0).contiguous(), kv_lens=i32([20, 16]), q_start=i32([0, 1, 2, 3]), q_lens=one, max_q=1, beams=2,
+                  causal=True, scale=None)
+    select = dict(logits=x, scores=s, finished=f, eos=2, history=h, step=0, step_at=i32([3]))
+    reorder = dict(parents=torch.tensor([[1, 1], [0, 0]], device=DEV), kv_lens=i32([20, 16]), tables=tables.clone(), cache=torch.stack([kc, vc]))
+    return {"plan_pages": plan, "write_pages": dict(k=k, v=v, key_cache=kc, value_cache=vc, slots=torch.tensor([3, -1, 40, 100], device=DEV)), "attend_pages": attend, "select_beams": select,
+            "reorder_pages": reorder, "copy_pages": dict(copies=i32([[0, 4, 5]]), cache=torch.stack([kc, vc]))}
+
+
+@pytest.mark.parametrize("form", ["default", "out"])
+@pytest.mark.parametrize("name", ["plan_pages", "write_pages", "attend_pages", "select_beams", "reorder_pages", "copy_pages"])
+def test_a_call_writes_what_its_schema_marks_and_nothing_else(name, form):
+    D()._lib()
+    packet = getattr(torch.ops.mmf_amd_decode, name)
+    if form not in packet.overloads():
+        pytest.skip("no such form")
+    args, want = form_args()[name], None
+    if form == "out":
+        outs = [a.name for a in packet.out._schema.arguments if a.kwarg_only]
+        want = packet.default(**form_args()[name])
+        want = want if isinstance(want, (tuple, list)) else (want,)
+        assert len(want) == len(outs)
+        args.update({n: torch.full_like(w, True if w.dtype == torch.bool else 77) for n, w in zip(outs, want)})
+    before = {n: t.clone() for n, t in args.items() if torch.is_tensor(t)}
+    got = getattr(packet, form)(**args)
+    written = {a.name for a in getattr(packet, form)._schema.arguments if a.alias_info is not None and a.alias_info.is_write}
+    changed = {n for n, t in before.items() if not torch.equal(t, args[n])}
+    assert changed <= written, changed - written
+    if form == "out":
+        assert got is None and all(torch.equal(args[n], w) for n, w in zip(outs, want))
+    else:
+        results = [] if got is None else list(got) if isinstance(got, (tuple, list)) else [got]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in results if t.numel())
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))                       # results do not overlap
+        held = {args[n].untyped_storage().data_ptr() for n in before}
+        assert not any(t.untyped_storage().data_ptr() in held for t in results if t.numel())
