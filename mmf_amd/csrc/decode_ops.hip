@@ -130,6 +130,7 @@ DEVI void plan_row(const mmf_paged_plan_desc& d, int shift, const PlanGroup& g, 
             for (int i = tid; i < g.granted; i += nthr) {
                 const int pos = g.kv + i, j = pos >> shift;
                 const int page = j >= lo ? from[-j] : part;
+                if (page < 0) flag_page_error();                  // (the token has no slot; a page beyond the pool is the write's to see)
                 d.slots[start + i] = page < 0 ? -1 : ((int64_t)page << shift) + (pos & below);
                 d.positions[start + i] = pos;
             }
@@ -138,6 +139,7 @@ DEVI void plan_row(const mmf_paged_plan_desc& d, int shift, const PlanGroup& g, 
             if (fork && j == lo) {
                 int* c = d.copies + 3 * (size_t)r;
                 c[0] = part; c[1] = page; c[2] = g.kv & below;
+                if (part < 0) flag_page_error();                  // (nothing to copy from)
             }
             table[j] = page;
             owned[j] = gets ? page : -1;                          // a shared block belongs to the group's first row

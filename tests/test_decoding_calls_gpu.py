@@ -182,3 +182,43 @@ def test_a_call_writes_what_its_schema_marks_and_nothing_else(name, form):
         assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))                       # results do not overlap
         held = {args[n].untyped_storage().data_ptr() for n in before}
         assert not any(t.untyped_storage().data_ptr() in held for t in results if t.numel())
+
+
+# ---------------------------------------------------------------------------------------------
+# pages that are none: reported by whoever leaves them out
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("groups", [1, 300])
+@pytest.mark.parametrize("beams,shared,new", [(1, True, 1), (1, True, 40), (3, False, 1), (3, True, 2)])
+def test_a_plan_reports_tokens_whose_block_has_no_page(beams, shared, new, groups):
+    """Tokens that go on in a block whose table entry is -1 get no slot; those behind it have pages of their own.  In one launch and in two."""
+    from mmf_amd import _native as nat
+    page, P = 16, 6
+    tables = torch.full((groups * beams, P), -1, dtype=I32, device=DEV)
+    tables[:, 0] = torch.arange(groups * beams, dtype=I32, device=DEV)
+    per = 1 if shared else beams
+    free = torch.arange(1000, 1000 + 4 * groups * beams, dtype=I32, device=DEV)
+
+    def plan(t):
+        return D().plan_pages(torch.full((groups,), new, dtype=I32, device=DEV), torch.full((groups,), 5, dtype=I32, device=DEV), t, t.clone(), free.clone(), i32([free.numel()]),
+                              page_size=page, rows=groups * per * new, beams=beams, shared=shared)
+    good = plan(tables.clone())
+    assert not nat.take_index_error() and bool((good.slots >= 0).all()) and int(good.refused) == 0
+    bad = tables.clone()
+    bad[0, 0] = -1
+    p = plan(bad)
+    assert nat.take_index_error()
+    lost = min(new, page - 5)
+    want = good.slots.clone()
+    want[:lost] = -1
+    assert torch.equal(p.slots, want) and torch.equal(p.positions, good.positions) and torch.equal(p.q_lens, good.q_lens)
+
+
+def test_a_plan_reports_a_block_that_cannot_be_copied_and_free_pages_that_are_none():
+    from mmf_amd import _native as nat
+    t, o = i32([[-1, -1], [-1, -1]]), i32([[0, -1], [-1, -1]])          # the second beam shares the block and has to have a copy of it
+    p = D().plan_pages(i32([1]), i32([3]), t, o, i32([7, 8]), i32([2]), page_size=16, rows=2, beams=2)
+    assert nat.take_index_error()
+    assert p.copies.tolist() == [[-1, -1, -1], [-1, 8, 3]] and p.slots.tolist() == [-1, 8 * 16 + 3]
+    t = i32([[-1, -1]])
+    p = D().plan_pages(i32([1]), i32([0]), t, t.clone(), i32([7, -4]), i32([2]), page_size=16, rows=1)
+    assert nat.take_index_error() and p.slots.tolist() == [-1]
