@@ -674,7 +674,7 @@ __global__ __launch_bounds__(256) void reorder_tables_kernel(mmf_paged_reorder_d
         }
     }
     __syncthreads();
-    const int kv = max(d.kv_lens[g], 0), rest = kv & (d.page_size - 1), part = rest ? kv / d.page_size : -1, cols = LIST / W;
+    const int told = d.kv_lens[g], kv = max(told, 0), rest = kv & (d.page_size - 1), part = rest ? kv / d.page_size : -1, cols = LIST / W;
     const int* from = d.tables + (size_t)g * W * d.blocks;
     int* to = d.tables_out + (size_t)g * W * d.blocks;
     for (int j0 = 0; j0 < d.blocks; j0 += cols) {                 // through LDS, many columns at a time: in place as well
@@ -694,9 +694,11 @@ __global__ __launch_bounds__(256) void reorder_tables_kernel(mmf_paged_reorder_d
             c[0] = copied[tid];
             c[1] = copy ? pages[tid * cols + part - j0] : -1;
             c[2] = copy ? rest : -1;
+            if (copy && (c[0] < 0 || c[1] < 0)) flag_page_error();               // (left out; a page beyond the pool is the copy's to see)
         }
         __syncthreads();
     }
+    if (tid == 0 && (told < 0 || kv > (int64_t)d.blocks * d.page_size)) flag_page_error();       // (a length that the table has no blocks for: full blocks only)
     if ((part < 0 || part >= d.blocks) && tid < 3 * W) d.copies[3 * (size_t)g * W + tid] = -1;
 }
 

@@ -222,3 +222,30 @@ def test_a_plan_reports_a_block_that_cannot_be_copied_and_free_pages_that_are_no
     t = i32([[-1, -1]])
     p = D().plan_pages(i32([1]), i32([0]), t, t.clone(), i32([7, -4]), i32([2]), page_size=16, rows=1)
     assert nat.take_index_error() and p.slots.tolist() == [-1]
+
+
+@pytest.mark.parametrize("case,reports", [("good", False), ("no source", True), ("no destination", True), ("no page, no copy", False), ("too long", True), ("negative", True),
+                                          ("full", False)])
+def test_a_reorder_reports_copies_without_a_page_and_lengths_without_a_block(case, reports):
+    from mmf_amd import _native as nat
+    cache = torch.randn(8, 2, 16, 64, device=DEV)
+    tables = [[0, 1], [2, 3], [4, 5]]
+    parents, kv = [[0, 0, 2]], 20                              # the second child of beam 0 takes beam 1's page
+    if case == "no source":
+        tables[0][1] = -1
+    elif case == "no destination":
+        tables[1][1] = -5
+    elif case == "no page, no copy":
+        parents, tables[2][1] = [[1, 0, 2]], -1
+    elif case in ("too long", "negative", "full"):
+        kv = {"too long": 33, "negative": -3, "full": 32}[case]
+    before, want = cache.clone(), cache.clone()
+    if case == "good":
+        want[3, :, :4] = before[1, :, :4]
+    got = D().reorder_pages(torch.tensor(parents, device=DEV), i32([kv]), i32(tables), cache)
+    assert nat.take_index_error() == reports
+    assert torch.equal(cache, want)
+    last = 1 if case in ("good", "no source", "no destination") else None               # the block that goes on being written, if there is one
+    for w, p in enumerate(parents[0]):
+        source = [0, 1, 2][w] if last else p
+        assert got[w].tolist() == [tables[p][0], tables[source][1]]
