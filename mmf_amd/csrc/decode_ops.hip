@@ -733,12 +733,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 extern "C" {
 
-int mmf_decode_take_error(void) {
-    int v = 0;
-    if (hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_page_error), sizeof(int)) != hipSuccess) { mmf_amd_set_error("take_index_error: copy failed"); return -1; }
-    if (v) { const int z = 0; (void)hipMemcpyToSymbol(HIP_SYMBOL(g_page_error), &z, sizeof(int)); }
-    return v;
-}
+int mmf_decode_take_error(void) { return take_page_error(); }
 
 int64_t mmf_paged_plan_ws_bytes(int groups, int beams) {
     return groups > 0 && beams > 0 ? (int64_t)groups * (int64_t)sizeof(PlanGroup) + 16 : 0;
@@ -757,6 +752,7 @@ int mmf_paged_plan(const mmf_paged_plan_desc* d, void* stream) {
     const int64_t walked = (int64_t)d->rows * (d->shared ? d->beams : 1);      // (every row of a shared group fills its table; rows of many tokens: fewer than a thread each)
     const bool one = walked <= 1024 || (walked <= 4 * rows && rows <= 4 * PLAN_THREADS);
     const int shift = __builtin_ctz(d->page_size);
+    page_kernels_used();
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(rows <= 256 ? 256 : PLAN_THREADS), 0, (hipStream_t)stream, *d, shift, (int)one);
     MMF_CHECK_LAUNCH();
     if (!one) {                                                   // a workgroup per row, and a few where rows have many tokens on average: some have many times that
@@ -780,6 +776,7 @@ int mmf_paged_write(const mmf_paged_write_desc* d, void* stream) {
     const int64_t per_token = 2ll * d->kv_heads * d->head_dim / (wide ? unit : 1), blocks = (d->tokens * per_token + 255) / 256;
     MMF_CHECK_ARG(per_token <= 0x3fffffff && blocks <= 0x7fffffff, "paged_write: too many elements for one call");
     const dim3 grid((unsigned)blocks);
+    page_kernels_used();
     if (wide) hipLaunchKernelGGL(paged_write_kernel<uint4>, grid, dim3(256), 0, (hipStream_t)stream, *d, es, (int)per_token);
     else if (es == 4) hipLaunchKernelGGL(paged_write_kernel<uint32_t>, grid, dim3(256), 0, (hipStream_t)stream, *d, es, (int)per_token);
     else hipLaunchKernelGGL(paged_write_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, *d, es, (int)per_token);
@@ -804,6 +801,7 @@ static int beam_select(const mmf_beam_select_desc* d, const int32_t* step_at, vo
     const int segments = beam_segments(d->groups * d->beams, d->vocab, d->is_f32 != 0, &length);
     const dim3 grid(segments, d->groups * d->beams);
     const bool wide = ((uintptr_t)d->logits & 3) == 0 && (d->ld & 1) == 0;
+    page_kernels_used();
     if (d->is_f32) hipLaunchKernelGGL((beam_rows_kernel<float, true>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
     else if (wide) hipLaunchKernelGGL((beam_rows_kernel<bf16, true>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
     else hipLaunchKernelGGL((beam_rows_kernel<bf16, false>), grid, dim3(256), 0, (hipStream_t)stream, *d, segments, length);
@@ -824,6 +822,7 @@ int mmf_paged_reorder(const mmf_paged_reorder_desc* d, void* stream) {
     MMF_CHECK_ARG(d && d->parents && d->kv_lens && d->tables && d->tables_out && d->copies, "paged_reorder: null operand");
     MMF_CHECK_ARG(d->groups > 0 && d->beams >= 1 && d->beams <= MMF_BEAMS_MAX && d->blocks > 0, "paged_reorder: bad shape");
     MMF_CHECK_ARG(d->page_size >= 1 && d->page_size <= MMF_PAGE_MAX && (d->page_size & (d->page_size - 1)) == 0, "paged_reorder: page_size is a power of two up to 1024");
+    page_kernels_used();
     hipLaunchKernelGGL(reorder_tables_kernel, dim3(d->groups), dim3(256), 0, (hipStream_t)stream, *d);
     MMF_CHECK_LAUNCH();
     return 0;
@@ -837,6 +836,7 @@ int mmf_paged_copy(const mmf_paged_copy_desc* d, void* stream) {
     const bool wide = aligned16(d->cache) && d->head_dim % unit == 0 && d->plane_stride % unit == 0 && d->page_stride % unit == 0 && d->head_stride % unit == 0 &&
                       d->pos_stride % unit == 0;
     const dim3 grid(d->rows, d->planes);
+    page_kernels_used();
     if (wide) hipLaunchKernelGGL(copy_pages_kernel<uint4>, grid, dim3(256), 0, (hipStream_t)stream, *d, es);
     else if (es == 4) hipLaunchKernelGGL(copy_pages_kernel<uint32_t>, grid, dim3(256), 0, (hipStream_t)stream, *d, es);
     else hipLaunchKernelGGL(copy_pages_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, *d, es);

@@ -892,12 +892,7 @@ template <typename T, int D> int launch(const mmf_paged_attn_desc* d, const Shap
 
 extern "C" {
 
-int mmf_paged_attention_take_error(void) {
-    int v = 0;
-    if (hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_page_error), sizeof(int)) != hipSuccess) { mmf_amd_set_error("take_index_error: copy failed"); return -1; }
-    if (v) { const int z = 0; (void)hipMemcpyToSymbol(HIP_SYMBOL(g_page_error), &z, sizeof(int)); }
-    return v;
-}
+int mmf_paged_attention_take_error(void) { return take_page_error(); }
 
 int64_t mmf_paged_attention_ws_bytes(const mmf_paged_attn_desc* d) {
     if (!d || d->kv_heads <= 0 || d->heads < d->kv_heads || d->max_q < 1 || d->beams < 1) return 0;
@@ -922,6 +917,7 @@ int mmf_paged_attention(const mmf_paged_attn_desc* d, void* stream) {
                   "paged_attention: a page within 2 GiB, pages within 4 GiB of each other");
     if (d->tokens == 0) return 0;
     const Shape s = shape_of(d);
+    page_kernels_used();
     MMF_CHECK_ARG(s.ws == 0 || (d->ws && ((uintptr_t)d->ws & 15) == 0), "paged_attention: null workspace");
     if (d->is_f32) return d->head_dim == 64 ? launch<float, 64>(d, s, (hipStream_t)stream) : launch<float, 128>(d, s, (hipStream_t)stream);
     return d->head_dim == 64 ? launch<bf16, 64>(d, s, (hipStream_t)stream) : launch<bf16, 128>(d, s, (hipStream_t)stream);

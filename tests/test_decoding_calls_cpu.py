@@ -143,3 +143,18 @@ def test_a_plan_takes_a_whole_plan_of_results():
         bad[i] = z(11, dt=bad[i].dtype)
         with pytest.raises(RuntimeError, match="out.%s must be" % name):
             d.plan_pages(**args, out=bad)
+
+
+# ---------------------------------------------------------------------------------------------
+# errors between steps
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("entry", ["mmf_decode_take_error", "mmf_paged_attention_take_error"])
+def test_errors_of_kernels_that_never_ran_are_not_fetched(entry):
+    """Without a GPU a copy from the device fails (-1): a process that has launched none of these kernels makes none."""
+    import subprocess
+    import sys
+
+    from mmf_amd import _native as nat
+    code = "import ctypes; print(ctypes.CDLL(%r).%s())" % (nat.LIB_PATH, entry)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip() == "0", (r.stdout, r.stderr)

@@ -249,3 +249,31 @@ def test_a_reorder_reports_copies_without_a_page_and_lengths_without_a_block(cas
     for w, p in enumerate(parents[0]):
         source = [0, 1, 2][w] if last else p
         assert got[w].tolist() == [tables[p][0], tables[source][1]]
+
+
+# ---------------------------------------------------------------------------------------------
+# errors between steps
+# ---------------------------------------------------------------------------------------------
+def test_replays_report_as_often_as_they_meet_a_bad_page():
+    from mmf_amd import _native as nat
+    a = form_args()
+    write, attend = a["write_pages"], a["attend_pages"]
+    attend.pop("causal"), attend.pop("scale")
+    D().write_pages(**write)
+    D().attend_pages(**attend)
+    assert not nat.take_index_error()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        D().write_pages(**write)
+        D().attend_pages(**attend)
+    good, table = write["slots"].clone(), attend["tables"].clone()
+    for turn in range(6):
+        write["slots"].copy_(good + (10 ** 6 if turn % 3 == 1 else 0))
+        attend["tables"].copy_(table + (100 if turn % 3 == 2 else 0))
+        torch.cuda.synchronize()
+        assert not nat.take_index_error()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert nat.take_index_error() == (turn % 3 != 0), turn
+        assert not nat.take_index_error()
