@@ -277,3 +277,44 @@ def test_replays_report_as_often_as_they_meet_a_bad_page():
         torch.cuda.synchronize()
         assert nat.take_index_error() == (turn % 3 != 0), turn
         assert not nat.take_index_error()
+
+
+# ---------------------------------------------------------------------------------------------
+# groups of beams that do not fill a workgroup evenly, calls with nothing to do, lists of free pages that are not what they say
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("beams,heads,kv_heads,new,kv,shared", [(5, 16, 2, 1, [150, 33, 1], 32), (3, 16, 1, 1, [70, 200], 64), (7, 12, 2, 1, [700, 40], 512), (5, 6, 2, 2, [90, 17], 16),
+                                                               (32, 24, 8, 1, [40], 16), (3, 32, 1, 1, [600, 100], 0)])
+def test_beams_that_a_workgroup_takes_in_uneven_parts(dtype, beams, heads, kv_heads, new, kv, shared):
+    from tests.test_decoding_gpu import attend_case, attend_check
+    attend_check(attend_case(kv, [min(new, n) for n in kv], beams=beams, heads=heads, kv_heads=kv_heads, dtype=dtype, shared=shared), beams=beams)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("max_q", [1, 40])
+@pytest.mark.parametrize("kv", [[70, 20], [3000, 700], [0, 0]])
+def test_attention_without_a_new_token_leaves_its_result_alone(dtype, max_q, kv):
+    from tests.test_decoding_gpu import attend_case
+    c = attend_case(kv, [0, 0], heads=4, kv_heads=2, dtype=dtype, gaps=50)
+    out = torch.full_like(c["q"], 7.0)
+    D().attend_pages(c["q"], c["key_cache"], c["value_cache"], c["tables"], c["kv_lens"], c["q_start"], c["q_lens"], max_q=max_q, out=out)
+    assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("told,top", [(9, 5), (-3, 0)])
+def test_a_plan_reports_a_stack_that_is_longer_than_its_list(told, top):
+    from mmf_amd import _native as nat
+    t = torch.full((1, 4), -1, dtype=I32, device=DEV)
+    p = D().plan_pages(i32([20]), i32([0]), t, t.clone(), i32([10, 11, 12, 13, 14]), i32([told]), page_size=16, rows=20)
+    assert nat.take_index_error()
+    assert p.free_top.tolist() == [top - 2 if top else 0] and p.refused.tolist() == [0 if top else 1]
+    assert t.tolist() == ([[14, 13, -1, -1]] if top else [[-1] * 4])
+
+
+def test_a_plan_reports_pages_that_come_back_twice():
+    from mmf_amd import _native as nat
+    t = i32([[0, 1], [2, 3]])
+    free = i32([7, 8, -1])
+    p = D().plan_pages(i32([-1, -1]), i32([32, 32]), t, t.clone(), free, i32([2]), page_size=16, rows=1)      # four pages come back where one fits
+    assert nat.take_index_error()
+    assert p.free_top.tolist() == [3] and free.tolist() == [7, 8, 0] and p.kv_lens.tolist() == [0, 0]
