@@ -24,6 +24,7 @@ void check(const Tensor& t, const char* name, at::ScalarType dt) {
     NEED(t.scalar_type() == dt, name, " must be ", dt, ", got ", t.scalar_type());
     NEED(!(t.requires_grad() && at::GradMode::is_enabled()), name, " requires a gradient: decoding is forward only (torch.no_grad)");
     NEED(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), name, " carries a tangent: decoding has no derivative in forward mode");
+    NEED(!t.is_neg(), name, " is a negated view, whose memory holds other values (resolve_neg)");
 }
 void check_float(const Tensor& t, const char* name) {
     NEED(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, name, " must be bfloat16 or float32, got ", t.scalar_type());

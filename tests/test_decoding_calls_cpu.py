@@ -158,3 +158,16 @@ def test_errors_of_kernels_that_never_ran_are_not_fetched(entry):
     code = "import ctypes; print(ctypes.CDLL(%r).%s())" % (nat.LIB_PATH, entry)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.strip() == "0", (r.stdout, r.stderr)
+
+
+# ---------------------------------------------------------------------------------------------
+# views whose values are not their memory
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("call,name", [(c, n) for c, (_, _, names) in calls().items() for n in names])
+def test_negated_views_are_refused(call, name):
+    f, args, _ = calls()[call]
+    view = torch._neg_view(args[name])
+    with pytest.raises(RuntimeError, match="%s is a negated view" % name):
+        f(**dict(args, **{name: view}))
+    with pytest.raises(RuntimeError, match="HBM"):
+        f(**dict(args, **{name: view.resolve_neg()}))
