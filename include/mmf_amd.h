@@ -789,7 +789,9 @@ int mmf_paged_write(const mmf_paged_write_desc* d, void* stream);
  *   out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j],  j < kv (causal: j <= kv - q_len + i),  query head h reads key head h / (heads / kv_heads).
  * Row r: queries q_start[r] .. + q_lens[r / beams], keys kv_lens[r / beams].  A token that sees no key gives zeros; rows of `out` no request names are left
  * as they were.  head_dim 64 or 128; bf16 (probabilities rounded to bf16 for the second product) or fp32 throughout; softmax statistics and sums fp32.
- * max_q: no request has more new tokens.  ws: mmf_paged_attention_ws_bytes(d) bytes, 16-byte aligned (0: none needed). */
+ * max_q: no request has more new tokens.  ws: mmf_paged_attention_ws_bytes(d) bytes, 16-byte aligned (0: none needed), for the partial results of requests that are split;
+ * it goes by what the tables have room for, not by the lengths: none for tables of up to 512 keys, else with head_dim 64 / 128 9 / 17 MB where max_q rows of a key head's
+ * query heads are at most 32, and 52 / 102 MB where they are more.  Calls that may run at the same time need one each. */
 typedef struct mmf_paged_attn_desc {
     const void* q; int64_t q_row, q_head;
     const void* k_cache; const void* v_cache; int64_t page_stride, head_stride, pos_stride;
@@ -820,7 +822,8 @@ int mmf_beam_select(const mmf_beam_select_desc* d, void* stream);
  * the rows of the parents come back without the new tokens. */
 int mmf_beam_select_at(const mmf_beam_select_desc* d, const int32_t* step, void* stream);
 /* Tables after a selection: row w of a group becomes row parents[w]; the first child of a row keeps its unfinished block's page, every other child gets the page
- * of a row without children and a line in copies [groups * beams, 3] (source, destination, tokens; else -1) for mmf_paged_copy.  tables_out may be tables. */
+ * of a row without children and a line in copies [groups * beams, 3] (source, destination, tokens; else -1) for mmf_paged_copy.  tables_out may be tables.
+ * Pages stay with the row that took them (`owned` of mmf_paged_plan) until their group is done, also those of full blocks that no row's table names any more. */
 typedef struct mmf_paged_reorder_desc {
     const int64_t* parents; const int32_t* kv_lens; const int32_t* tables; int32_t* tables_out; int32_t* copies;
     int groups, beams, blocks, page_size;

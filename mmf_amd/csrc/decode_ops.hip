@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256) void plan_rows_kernel(mmf_paged_plan_desc d, i
 
 // ------------------------------------------------------------------------------------------------
 // new keys and values into their slots.  Every byte moves once each way, and memory bounds it: 16384 rows of 8 heads of 128 in bf16, 27 us for 121 MB; 160 rows of 12 heads
-// of 64: 2.3 us, an empty launch.  A thread moves one VT: 16 bytes, or one element where a row does not start on 16 bytes (134 MB that caches hold: 22 us by 16 bytes,
+// of 64: 2.8 us, an empty launch.  A thread moves one VT: 16 bytes, or one element where a row does not start on 16 bytes (134 MB that caches hold: 22 us by 16 bytes,
 // 122 by elements).
 // ------------------------------------------------------------------------------------------------
 template <typename VT>
@@ -275,8 +275,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(mmf_paged_write_desc d
 // maximum, its sum of exponentials and its W largest; a second one merges the segments and beams of a group.  Both pick W out of N in the same way: of the maxima of
 // 64 groups of threads the W-th largest is a bar that at least W values reach, and few more do; those are ranked by counting.
 //
-// 128 rows of 128000 logits in bf16, 8 beams: 15 us for the rows (33 MB; half of it arithmetic, 16 instructions a logit of which the exponential and its correction are 7,
-// that starts when most loads have landed) and 10 for the merge; 160 rows of 5050 in fp32, 5 beams: 6.3 and 6.9 us.  The merge is a chain of trips to memory and to
+// 128 rows of 128000 logits in bf16, 8 beams: 15 us for the rows (33 MB; vector instructions, 23 a logit of which the exponential and its correction are 7, issue in 40 % of
+// its cycles, and start when most loads have landed) and 10 for the merge; 160 rows of 5050 in fp32, 5 beams: 6.3 and 7.5 us.  The merge is a chain of trips to memory and to
 // LDS by a workgroup per group: what does not wait for the sums (lists, segments, the history's first columns) is read first.
 // ------------------------------------------------------------------------------------------------
 constexpr double NEG_INF = -__builtin_huge_val();

@@ -16,10 +16,14 @@
 // What bounds it, and what it measured (MI355X; a copy of 1 GiB reaches 5.18 TB/s, a bf16 product of 8192^3 1262 TFLOP/s, an fp32 one of 4096^3 139):
 //   long caches   8 requests of 16384 .. 65536 keys, 32 heads on 8, head_dim 128, one token: 191 us, 5.3 TB/s of pages.  Memory.
 //   steps         32 groups of 5 beams, 120 .. 181 keys of which the prompt's pages are shared, 12 heads of 64: 11.9 us for 21.5 MB.  The chain lengths, table,
-//                 first tile, four tiles, meeting of the waves; with every beam reading the shared pages itself 25.3 us.
-//   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 340 us, 794 TFLOP/s (333 on another card).  Products (512 cycles per 32 keys of a wave) and vector instructions (500) of
-//                 the two waves that a SIMD holds; without exponentials it takes 320 us, without staging 293, without barriers too 280.
-//   fp32 prompts  32 prompts of 70 .. 170 tokens, 12 heads of 64: 35.6 us.  The products of the longest prompts (3.5 us per 32 keys for two waves on a SIMD) behind 10 us
+//                 first tile, four tiles, meeting of the waves; with every beam reading the shared pages itself 25.3 us.  The fp32 pool: 27.3 us for 43 MB.
+//   fp32 tokens   8 requests of 2048 .. 8192 keys, 32 heads on 8, one token: 110.8 us at head_dim 128 (2.3 TB/s), 51.5 at 64 (2.5).  A tile's load waits for the score
+//                 products of the one before, and a product takes 32 rows where 4 are the request's.
+//   chunks        270 GFLOP over caches, 32 heads on 8, head_dim 128: 333 us, 808 TFLOP/s (340 on another card), 15 of it to join runs.  Products (512 cycles per 32
+//                 keys of a wave) and vector instructions (545) of the two waves that a SIMD holds: the matrix units are busy in 37 % of the cycles, vector instructions
+//                 issue in 44 %.  Of 340 us, copies without exponentials took 320, without staging 293, without barriers too 280.  At head_dim 64 (135 GFLOP) 194 us,
+//                 694 TFLOP/s; 32 prompts of 70 .. 170 tokens, 12 heads of 64, not causal: 15.2 us.
+//   fp32 prompts  the same 32 prompts: 35.6 us.  The products of the longest prompts (3.5 us per 32 keys for two waves on a SIMD) behind 10 us
 //                 of lengths, plan, queries, first tile and output.
 #include "common.h"
 #include "mmf_amd.h"

@@ -14,7 +14,8 @@ A cache pool is [pages, kv_heads, page_size, head_dim] (any strides with contigu
 in groups of `beams` rows of the same length; a block table [groups * beams, blocks] int32 names the page of every block of a row.  Lengths stay on the device: no
 call here waits for the GPU, and every call can be captured into a hipGraph (its numbers with it: a selection that is replayed takes its `step` from the device).  An
 index outside its table (a page, a slot, a parent, a step) is left out and reported by `mmf_amd._native.take_index_error()`.  Forward only: tensors that require
-gradients are refused while gradients are on, and so are those that carry a tangent of forward-mode differentiation."""
+gradients are refused while gradients are on, and so are those that carry a tangent of forward-mode differentiation.  The
+operators have no form without data, so torch.compile does not trace through them: call them outside of what it compiles."""
 import os
 from collections import namedtuple
 
@@ -61,7 +62,8 @@ def plan_pages(q_lens, kv_lens, tables, owned, free_pages, free_top, *, page_siz
 
     A group is served whole or waits (no page, no slot, q_lens 0): when its tokens do not fit its table row or `rows`, or when it and the groups before it need
     more pages than are free.  Not shared, a row that still shares the block it goes on writing gets a page of its own and a line in `copies`: call
-    `copy_pages(plan.copies, cache)` before the write.  `out`: a PagePlan whose tensors take the results; its kv_lens and free_top may be the inputs."""
+    `copy_pages(plan.copies, cache)` before the write.  Lengths change by plans alone (a length set back by hand loses the pages behind it).
+    `out`: a PagePlan whose tensors take the results; its kv_lens and free_top may be the inputs."""
     if out is None:
         return PagePlan(*_lib().plan_pages(q_lens, kv_lens, tables, owned, free_pages, free_top, page_size, rows, beams, shared), 1 if shared else beams)
     if len(out) < 8:
@@ -86,7 +88,10 @@ def attend_pages(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, *,
     new tokens, written before, are the last.  causal: a new token sees the keys up to itself; else all of them.  tables int32 [requests, blocks]
     (contiguous rows); kv_lens, q_lens int32 [requests // beams], q_start int32 [requests].  max_q: no request has more new tokens (tokens beyond are left out and
     reported).  scale: default head_dim ** -0.5.  A token that sees no key gives zeros; rows of `out` that no request names are left as they are (undefined
-    where `out` is made here).  `out` may be q.  A page outside the pool reads as zeros and is reported."""
+    where `out` is made here).  `out` may be q.  A page outside the pool reads as zeros and is reported.
+
+    Requests longer than 512 keys may be split over the chip.  A call whose tables have room for such ones takes a workspace from torch's allocator, whatever the lengths are: 9 MB
+    at head_dim 64 and 17 at 128 for single tokens (up to 32 rows of query heads and new tokens per key head), 52 and 102 MB for chunks; a captured call keeps its own."""
     if out is None:
         return _lib().attend_pages(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, max_q, beams, causal, scale)
     _lib().attend_pages_out(q, key_cache, value_cache, tables, kv_lens, q_start, q_lens, max_q, beams, causal, scale, out=out)
@@ -121,7 +126,10 @@ def reorder_pages(parents, kv_lens, tables, cache, *, out=None):
     parents int64 [groups, beams]; kv_lens int32 [groups]: tokens in the cache; tables int32 [groups * beams, blocks]; cache [..., pages, kv_heads, page_size,
     head_dim]: every pool the tables are for (keys and values of all layers), leading dimensions as one contiguous run of planes.  Full blocks are shared by the children
     of a beam.  The block that goes on being written stays with the first child; the other children take the pages of beams without children and get its
-    tokens copied in.  Returns the new tables (`out` may be `tables`)."""
+    tokens copied in.  Returns the new tables (`out` may be `tables`).
+
+    Pages stay with the row that took them until their group is done, also full ones that no table names any more: a pool has to hold, for each group, the blocks of its
+    prompt and `beams` times the blocks written since, not just the pages that are still read."""
     if out is None:
         return _lib().reorder_pages(parents, kv_lens, tables, cache)
     _lib().reorder_pages_out(parents, kv_lens, tables, cache, out=out)
@@ -135,7 +143,8 @@ def copy_pages(copies, cache):
 
 
 class PagedCache:
-    """Pool, block tables, free list and lengths of a decoder with `layers` layers for `groups` requests of `beams` rows; every update is in place, so that a
+    """Pool, block tables, free list and lengths of a decoder with `layers` layers for `groups` requests of `beams` rows of up to `max_len` tokens.  `pages`: those that any
+    course of decoding can take (groups * beams * blocks); with fewer, groups may have to wait (`plan.refused`).  Every update is in place, so that a
     step can be captured once and replayed (with `select_beams(..., step=at)`, `at` an int32 [1] tensor that the step advances).
 
         cache = PagedCache(layers, groups, beams, max_len, kv_heads=12, head_dim=64)
