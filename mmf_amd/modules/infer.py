@@ -38,7 +38,9 @@ def layer_rows(layer, x2, cache, B, rows_per_sample, cache_rows, row0, Sk, key_m
     nat.attention_fwd(q, cache[:, H:], cache[:, 2 * H:], 3 * H, 3 * H, 3 * H, key_mask_add, ctxt, H, lse, B, heads, R, Sk,
                       1.0 / math.sqrt(H // heads), head_dim=H // heads, q_batch_rows=cache_rows, kv_batch_rows=cache_rows,
                       mask_batch_stride=cache_rows if key_mask_add is not None else 0)
-    return _finish_rows(layer, x2, ctxt)
+    # (one launch: the skinny split-K path — a workspace allocation and a second kernel per call — is for the training heads' long
+    # reductions, not for a host-bound decoding loop; bit 18 of debug_flags keeps the long-K GEMM of the feed-forward on the single-kernel path)
+    return _finish_rows(layer, x2, ctxt, nat.GEMM_NO_SKINNY)
 
 
 def new_cache(B, cache_rows, H, layers, device):
@@ -68,14 +70,11 @@ def layer_rows_paged(layer, x2, cache, index, plan, max_q, causal, out_rows=None
     if f32:
         a_out = F32P.dense_residual_ln(ctxt, x2, so.dense.weight, so.dense.bias, so.LayerNorm.weight, so.LayerNorm.bias, so.LayerNorm.eps)
         return F32P.feed_forward(a_out, it.dense.weight, it.dense.bias, ot.dense.weight, ot.dense.bias, ot.LayerNorm.weight, ot.LayerNorm.bias, ot.LayerNorm.eps)
-    return _finish_rows(layer, x2, ctxt)
+    return _finish_rows(layer, x2, ctxt, nat.GEMM_NO_SKINNY)
 
 
-def _finish_rows(layer, x2, ctxt):
-    """Output projection + residual + LayerNorm, GELU feed-forward + residual + LayerNorm on [M, H] bf16 rows.
-
-    The long-K GEMM of the feed-forward stays one launch: the skinny split-K path, a workspace allocation and a second kernel per call, is for the training heads' long
-    reductions and not for a host-bound decoding loop.  It takes 64 rows at most, so for the packed rows of a batch's prompts the flag changes nothing."""
+def _finish_rows(layer, x2, ctxt, down_flags):
+    """Output projection + residual + LayerNorm, GELU feed-forward + residual + LayerNorm on [M, H] bf16 rows; down_flags: debug_flags of the long-K GEMM."""
     so, it, ot = layer.attention.output, layer.intermediate, layer.output
     M, H = x2.shape
     dev = x2.device
@@ -88,7 +87,7 @@ def _finish_rows(layer, x2, ctxt):
     nat.gemm(a_out, Fn.shadows.get(it.dense.weight), hh, M, I, H, H, H, I, bias=it.dense.bias.detach(), act=1)
     y2 = torch.empty(M, H, dtype=BF16, device=dev)
     nat.gemm(hh, Fn.shadows.get(ot.dense.weight), y2, M, H, I, I, I, H, bias=ot.dense.bias.detach(), resid=a_out, ldr=H,
-             debug_flags=nat.GEMM_NO_SKINNY)
+             debug_flags=down_flags)
     out = torch.empty(M, H, dtype=BF16, device=dev)
     nat.layernorm_fwd(y2, ot.LayerNorm.weight.detach(), ot.LayerNorm.bias.detach(), out, None, None, M, H, ot.LayerNorm.eps)
     return out
