@@ -70,6 +70,7 @@ def layer_rows_paged(layer, x2, cache, index, plan, max_q, causal, out_rows=None
     if f32:
         a_out = F32P.dense_residual_ln(ctxt, x2, so.dense.weight, so.dense.bias, so.LayerNorm.weight, so.LayerNorm.bias, so.LayerNorm.eps)
         return F32P.feed_forward(a_out, it.dense.weight, it.dense.bias, ot.dense.weight, ot.dense.bias, ot.LayerNorm.weight, ot.LayerNorm.bias, ot.LayerNorm.eps)
+    # (one launch here too: a step is the same host-bound loop, and the packed rows of a batch's prompts are more than the 64 that the skinny path takes)
     return _finish_rows(layer, x2, ctxt, nat.GEMM_NO_SKINNY)
 
 
