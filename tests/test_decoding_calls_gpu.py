@@ -155,13 +155,14 @@ def form_args():
             "reorder_pages": reorder, "copy_pages": dict(copies=i32([[0, 4, 5]]), cache=torch.stack([kc, vc]))}
 
 
-@pytest.mark.parametrize("form", ["default", "out"])
-@pytest.mark.parametrize("name", ["plan_pages", "write_pages", "attend_pages", "select_beams", "reorder_pages", "copy_pages"])
+FORMS = [(n, "default") for n in ("plan_pages", "write_pages", "attend_pages", "select_beams", "reorder_pages", "copy_pages")] + \
+        [(n, "out") for n in ("plan_pages", "attend_pages", "select_beams", "reorder_pages")]
+
+
+@pytest.mark.parametrize("name,form", FORMS)
 def test_a_call_writes_what_its_schema_marks_and_nothing_else(name, form):
     D()._lib()
     packet = getattr(torch.ops.mmf_amd_decode, name)
-    if form not in packet.overloads():
-        pytest.skip("no such form")
     args, want = form_args()[name], None
     if form == "out":
         outs = [a.name for a in packet.out._schema.arguments if a.kwarg_only]
